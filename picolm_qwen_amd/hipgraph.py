@@ -64,6 +64,7 @@ class Graph:
         if err is not None:
             if self.graph:
                 L.hipGraphDestroy(self.graph)
+                self.graph = C.c_void_p()
             raise err
         _check(rc, "hipStreamEndCapture")
         _check(L.hipGraphInstantiate(C.byref(self.exec), self.graph, None, None, 0), "hipGraphInstantiate")
