@@ -380,6 +380,119 @@ int pqa_set_batch_projection(pqa_ctx* ctx, int exact_kv);
  *    weights of 2 already put outputs past max-abs 2e-3 / rel 1e-2). */
 int pqa_set_prefill_precision(pqa_ctx* ctx, int split_q);
 
+/*
+ * ---- Paged cache: many sequences at once ----
+ *
+ * pqa_ctx holds one sequence in the reference's contiguous layout. A server of many requests
+ * keeps their keys and values in pages of a shared pool instead: a pqa_paged handle is the pool,
+ * a pqa_batch says which tokens of which sequences the next calls are about. No counterpart in
+ * the reference, which serves one sequence; norm, rotation, rounding and attention are its own
+ * (the block of cpp/model.hpp:326-418), so fp16 rows of a PQA_PAGED_F32 handle have the bits that
+ * pqa_decode writes.
+ *
+ * Layouts, all in the handle's device memory:
+ *   key_pages, val_pages  [n_layers][n_pages][n_kv_heads][page_size][head_dim], 2 bytes each
+ *   key_bounds            int8 [n_layers][n_pages][n_kv_heads][2][head_dim]
+ *   key_scales            float [n_layers][n_pages][n_kv_heads]
+ * Token rows: q [n][n_heads * head_dim], k and v [n][n_kv_heads * head_dim], the batch's new
+ * tokens sequence by sequence, with a distance between rows in elements (*_stride: a row of a
+ * wider array may hold q, k and v side by side). Any alignment of whole elements is taken; 16-byte
+ * rows are faster.
+ *
+ * Streams: calls run on the hipStream_t given as `stream` (NULL: the default stream), on the
+ * handle's device whatever device is current, and are asynchronous. Everything that uses one
+ * batch must be ordered (one stream, or events), pqa_batch_set included: the batch holds the
+ * tables and the workspace of its calls. Calls on different batches may overlap, captured ones as
+ * well, as long as no page that one of them writes is used by another.
+ * Capture: pqa_paged_append, _attend, _forward and _attend_sparse may be captured. A replay works
+ * on what the batch holds by then: set the batch again, write the new rows into the same
+ * buffers, replay. The buffers must hold the batch's max_tokens rows if the batch may grow.
+ * Threading: a handle and its batches are used by one host thread at a time. Errors:
+ * pqa_paged_last_error; a call that fails launches nothing.
+ */
+typedef struct pqa_paged pqa_paged;
+typedef struct pqa_batch pqa_batch;
+
+typedef enum {
+    PQA_PAGED_F32 = 0, /* fp32 token rows, fp16 pages: fp32-level results */
+    PQA_PAGED_F16 = 1, /* fp16 rows and pages */
+    PQA_PAGED_BF16 = 2 /* bf16 rows and pages */
+} pqa_paged_t;
+
+/*
+ * page_size: 16, 32, 64, 128 or 256 positions. head_dim: 64, 96, 128, 160, 192 or 256
+ * (PQA_ERR_UNSUPPORTED otherwise). n_heads a multiple of n_kv_heads. with_bounds: the handle keeps
+ * key bounds (pqa_paged_attend_sparse needs them). The memory is the caller's if its
+ * addresses are given (all of them; pages and bounds aligned to 16 bytes; it must outlive the
+ * handle), else the handle's own, zeroed. Made on the current device.
+ */
+int pqa_paged_create(pqa_paged** out, int n_layers, int n_pages, int page_size, int n_heads, int n_kv_heads, int head_dim,
+                     int type, int with_bounds, void* key_pages, void* val_pages, int8_t* key_bounds, float* key_scales);
+/* Waits for the device. Destroy the handle's batches first. */
+void pqa_paged_destroy(pqa_paged* p);
+const char* pqa_paged_last_error(const pqa_paged* p);
+/* The addresses of the cache's memory (bounds and scales NULL without bounds); any argument may be NULL. */
+int pqa_paged_memory(pqa_paged* p, void** key_pages, void** val_pages, int8_t** key_bounds, float** key_scales);
+
+/* Rotation of the first rot_dim elements of each head (even, at most head_dim; 0: none, as after
+ * creation) by HOST tables [max_pos][rot_dim / 2], paired as rope_style (pqa_rope_t) pairs a head
+ * of rot_dim elements. Tables for scaled positions are the caller's to compute. Positions end at
+ * max_pos: pqa_batch_set refuses longer sequences. Synchronous; batches are set again after it.
+ * Refused once an append has been captured. */
+int pqa_paged_set_rope(pqa_paged* p, int rope_style, int rot_dim, int max_pos, const float* rope_cos, const float* rope_sin);
+/* QK-RMSNorm weights of one layer, as pqa_set_qk_norm. Synchronous. */
+int pqa_paged_set_qk_norm(pqa_paged* p, int layer, const float* q_norm_w, const float* k_norm_w);
+
+/* A batch of at most max_seqs sequences with max_tokens new tokens in all and lengths up to
+ * max_len. Holds tables of 4 bytes per page of max_seqs sequences of max_len, and workspaces for
+ * cut rows: (2 x 16 x workgroups + up to 2 x 128 x workgroups) rows of head_dim + 2 floats, a
+ * workgroup or two per CU (8 + 68 MB at head size 128 on 256 CUs; none of the latter if
+ * max_tokens query rows of a KV head are 16 or fewer). */
+int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int max_tokens, int max_len);
+/* Waits for the device. */
+void pqa_batch_destroy(pqa_batch* b);
+/*
+ * What the next calls work on, from HOST arrays: sequence i has len[i] positions, of which
+ * the last n_new[i] are new (n_new[i] = 0: none), in pages[i * stride + j], j < ceil(len[i] /
+ * page_size). Sequences may share pages that they only read (a common prompt); a page that
+ * receives rows may be listed once only. PQA_ERR_RANGE for what exceeds the batch, the list or the
+ * rotation's tables, PQA_ERR_ARG for pages outside the pool and other contradictions; the batch
+ * then keeps what it held. The arrays are copied; the upload runs on `stream`. Not while
+ * the stream is captured.
+ */
+int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const int* len, const int* pages, int stride, void* stream);
+
+/* The new tokens' K and V into their pages (norm and rotation of K applied, rounded to the pages'
+ * type: fp16 with pqa_decode's rounding, bf16 to nearest even), q normed and rotated to q_out (may
+ * be q itself), and the key bounds of every page that received rows, if the handle keeps them.
+ * Rows behind the batch's last token are left as they were. */
+int pqa_paged_append(pqa_paged* p, pqa_batch* b, int layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride, void* stream);
+/* Causal attention of the new tokens, q as pqa_paged_append leaves it: token i of a sequence sees positions
+ * 0 .. len - n_new + i. Scale 1 / sqrt(head_dim). out may be q itself. Rows behind the
+ * batch's last token, and what pages hold behind a sequence's end, do not matter. */
+int pqa_paged_attend(pqa_paged* p, pqa_batch* b, int layer, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                     void* stream);
+/* Both: append, then attend; out also carries q in between. */
+int pqa_paged_forward(pqa_paged* p, pqa_batch* b, int layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                      const void* v, int64_t v_stride, void* out, int64_t out_stride, void* stream);
+/*
+ * pqa_paged_attend with a budget of `select` pages: each new token and KV head attends to the
+ * first `first` pages of its sequence, the `last` pages that end with the token's own, and those
+ * of the others with the largest scores (first + last <= select, last >= 1; all pages where there
+ * are no more than select). Written to chosen [n][n_kv_heads][select] (DEVICE), in
+ * ascending order as places in the sequence's page list, -1 behind the last.
+ * A page's score bounds the logits of its keys: with lo and hi the least and largest key of
+ * each dim over the page's rows (NaN left out) and e = floor(log2(max |lo|, |hi| over the dims)) within
+ * [-24, 24], the bounds hold floor(lo 2^(6-e)) and ceil(hi 2^(6-e)) within [-127, 127] and the scale
+ * 2^(e-6); a query head's row is rounded to the nearest (ties to even) likewise; the score is the
+ * largest over the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d), times both scales.
+ * It is exact, and of equal scores the lower page is taken. At most 32768 pages per sequence (captured:
+ * of the batch's max_len).
+ */
+int pqa_paged_attend_sparse(pqa_paged* p, pqa_batch* b, int layer, const void* q, int64_t q_stride, int select, int first,
+                            int last, int* chosen, void* out, int64_t out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

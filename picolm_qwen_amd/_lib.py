@@ -26,6 +26,9 @@ EXPORTS = [
     "pqa_set_qkv_weights", "pqa_qkv_project", "pqa_decode_x", "pqa_set_out_weights", "pqa_out_project",
     "pqa_attention_block", "pqa_qkv_project_batch", "pqa_prefill_x", "pqa_decode_noalloc",
     "pqa_out_project_batch", "pqa_prefill_block", "pqa_attention_block_host", "pqa_prefill_block_host",
+    "pqa_paged_create", "pqa_paged_destroy", "pqa_paged_last_error", "pqa_paged_memory", "pqa_paged_set_rope",
+    "pqa_paged_set_qk_norm", "pqa_batch_create", "pqa_batch_destroy", "pqa_batch_set", "pqa_paged_append",
+    "pqa_paged_attend", "pqa_paged_forward", "pqa_paged_attend_sparse",
 ]
 
 
@@ -121,8 +124,26 @@ def _bind(L: C.CDLL) -> C.CDLL:
     L.pqa_prefill_block.argtypes = [vp, i, i, i, vp, vp]
     L.pqa_attention_block_host.argtypes = [vp, i, i, vp, vp]
     L.pqa_prefill_block_host.argtypes = [vp, i, i, i, vp, vp]
+    i64 = C.c_int64
+    L.pqa_paged_create.argtypes = [C.POINTER(vp)] + [i] * 8 + [vp] * 4
+    L.pqa_paged_destroy.argtypes = [vp]
+    L.pqa_paged_destroy.restype = None
+    L.pqa_paged_last_error.argtypes = [vp]
+    L.pqa_paged_last_error.restype = C.c_char_p
+    L.pqa_paged_memory.argtypes = [vp] + [C.POINTER(vp)] * 4
+    L.pqa_paged_set_rope.argtypes = [vp, i, i, i, vp, vp]
+    L.pqa_paged_set_qk_norm.argtypes = [vp, i, vp, vp]
+    L.pqa_batch_create.argtypes = [vp, C.POINTER(vp), i, i, i]
+    L.pqa_batch_destroy.argtypes = [vp]
+    L.pqa_batch_destroy.restype = None
+    L.pqa_batch_set.argtypes = [vp, i, vp, vp, vp, i, vp]
+    L.pqa_paged_append.argtypes = [vp, vp, i] + [vp, i64] * 4 + [vp]
+    L.pqa_paged_attend.argtypes = [vp, vp, i] + [vp, i64] * 2 + [vp]
+    L.pqa_paged_forward.argtypes = [vp, vp, i] + [vp, i64] * 4 + [vp]
+    L.pqa_paged_attend_sparse.argtypes = [vp, vp, i, vp, i64, i, i, i, vp, vp, i64, vp]
     for name in EXPORTS:
-        if name not in ("pqa_stream", "pqa_last_error", "pqa_destroy", "pqa_rope_table"):
+        if name not in ("pqa_stream", "pqa_last_error", "pqa_destroy", "pqa_rope_table", "pqa_paged_destroy",
+                        "pqa_paged_last_error", "pqa_batch_destroy"):
             getattr(L, name).restype = C.c_int
     return L
 

@@ -1,0 +1,925 @@
+// Attention of a batch's new tokens over their sequences' pages:
+//   out = sum_j 2^(s_j - M) v_j / sum_j 2^(s_j - M),  s_j = (q . k_j) log2(e) / sqrt(d),
+// over the keys j up to the token's own position, in one pass with a running maximum M.
+//
+// Rows (query heads of one KV head, token by token) are packed 16 to a tile column:
+// S^T = K Q^T and O^T += V^T P^T on 16x16x32 matrix instructions, in whose layouts a lane's
+// scores are already its operand of the second product. Keys lie in blocks of 16, each within
+// one page ([page][kv_head][row][dim]) and so contiguous in memory; they arrive by direct
+// global->LDS loads, 16-byte chunk c of row r at slot c ^ x(r), which keeps the K operand reads
+// and the transposing V reads free of bank conflicts.
+//
+// Types: fp16 and bf16 rows enter the products as they are, P is rounded to the same type
+// (half a step, 2^-11 or 2^-8 of a weight; errors of many weights average out, and the output
+// is rounded to that type anyway). fp32 rows are split into two fp16 parts with 22
+// significant bits together (after an exact power of two), and so is P, the low parts' sums
+// apart: fp32-level results at twice the products. Scores, maxima and sums are fp32 throughout.
+//
+// Two kernels:
+//   narrow  up to 16 rows per sequence and KV head (single tokens): bound by reading K and V
+//           once. Waves take 32-key tiles in turn, each with two tiles of its own in flight,
+//           and meet in LDS. The batch's key tiles are cut into one run per workgroup, so
+//           that contexts of any mix of lengths keep all of them busy to the end.
+//   wide    more rows (chunks): bound by the products. 4 waves share each key tile (two
+//           buffers, one barrier per tile).
+// Rows whose keys were cut leave partial sums, which the last workgroup of these rows to
+// finish joins in a fixed order (results do not depend on which one that is).
+//
+// A split product can turn inf into NaN (inf * 0, inf - inf), and a masked key's V row still
+// enters the product with weight 0. A row whose result is not finite is therefore computed again by
+// slow_rows, in fp32 over its own keys alone.
+#include <algorithm>
+
+#include "pqa_paged_device.h"
+
+namespace pqa {
+
+namespace {
+
+constexpr float kNone = -3.0e38f;  // running maximum before the first key
+constexpr float kSlack = 4.0f;     // P is rescaled when a score passes the maximum by this many log2 units
+constexpr float kLow = 2048.0f;    // scale of P's low parts, to the exponents of the high ones
+
+struct PagedAttn {
+    const void* q;
+    void* out;
+    long long ldq, ldo;
+    const char* kp;  // the layer's pages
+    const char* vp;
+    const int* pages;
+    const int* items;  // PagedItem
+    const int* first;
+    const int* header;
+    float* part;
+    unsigned* counters;
+    const int* chosen;  // attention over chosen pages: [token][kv head][select], else null
+    const int* token_seq;
+    const int* seqs;  // PagedSeq
+    int select, wgs;
+    int g, n_kv, shift;
+    int qvec, ovec;  // rows may move as 16-byte vectors
+    float qscale;
+};
+
+// rows and keys of one piece of work
+struct Column {
+    int row0, rows, hist, table, kvh, r0;
+    int kend;         // keys that exist
+    const int* list;  // its chosen pages, or null: all pages of the sequence
+};
+
+constexpr int pow2_of(int ch) { return ch % 16 == 0 ? 16 : ch % 8 == 0 ? 8 : ch % 4 == 0 ? 4 : ch % 2 == 0 ? 2 : 1; }
+
+template <int HD>
+struct Geo {
+    static_assert(HD % 32 == 0 && HD <= 256, "whole 1 KB loads per block of 16 keys");
+    static constexpr int CH = HD / 8;         // 16-byte chunks per row
+    static constexpr int ROWB = HD * 2;
+    static constexpr int BLKB = 16 * ROWB;    // a block of 16 keys
+    static constexpr int PPB = BLKB / 1024;   // its 1 KB loads
+    static constexpr int P2 = pow2_of(CH);
+    static constexpr int PER = 16 / P2 > 0 ? 16 / P2 : 1;  // rows after which the bank of a chunk repeats
+    static constexpr int KS = HD / 32, DB = HD / 16;
+    static constexpr int QS = HD + 4;  // row stride of fp32 rows in LDS
+    __device__ static int xk(int r) { return (r / PER) & (P2 - 1); }
+    __device__ static int xv(int r) { return (2 * (r / PER)) & (P2 - 1); }
+};
+
+template <int TYPE>
+struct Ops;
+template <>
+struct Ops<PQA_PAGED_F16> {
+    typedef half8 V8;
+    static constexpr bool split = false;
+    static constexpr float scale = 2048.0f;  // of P: fp16's exponents reach down to 2^-25 of the largest weight
+    __device__ static floatx4 mul(V8 a, V8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Ops<PQA_PAGED_F32> : Ops<PQA_PAGED_F16> {
+    static constexpr bool split = true;
+};
+template <>
+struct Ops<PQA_PAGED_BF16> {
+    typedef bf16x8 V8;
+    static constexpr bool split = false;
+    static constexpr float scale = 1.0f;
+    __device__ static floatx4 mul(V8 a, V8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ int page_at(const PagedAttn& a, const Column& c, int i) {
+    const int j = c.list ? scalar_int(c.list, i) : i;
+    return scalar_int(a.pages, c.table + j);
+}
+
+// byte offset of the block of 16 keys at `pos` in page `page`
+template <int HD>
+__device__ __forceinline__ size_t block_offset(const PagedAttn& a, const Column& c, int page, int pos) {
+    return (size_t)((((unsigned)page * a.n_kv + c.kvh) << a.shift) + (pos & ((1 << a.shift) - 1))) * Geo<HD>::ROWB;
+}
+
+// element offset of packed row R in rows of distance ld
+template <int HD>
+__device__ __forceinline__ long long row_offset(const PagedAttn& a, const Column& c, int R, long long ld) {
+    const int tok = R / a.g;
+    return (long long)(c.row0 + tok) * ld + (c.kvh * a.g + R - tok * a.g) * HD;
+}
+
+// What a wave carries for one block of 16 rows; lane (c16, g16) holds row c16's.
+template <int TYPE, int HD>
+struct RowBlock {
+    typedef typename Ops<TYPE>::V8 V8;
+    static constexpr int KS = Geo<HD>::KS, DB = Geo<HD>::DB;
+    static constexpr bool split = Ops<TYPE>::split;
+    V8 q[KS], ql[split ? KS : 1];  // dims 32 ks + 8 g16 .. +7; high and low parts
+    float cs;                      // a raw score's factor to log2 units
+    int qpos;
+    float m, l;  // the maximum of the raw scores, and the lane's share of the sum
+    floatx4 o[DB], ol[split ? DB : 1];  // O^T: dims 16 db + 4 g16 .. +3; from P's high and low parts
+
+    __device__ void start(int pos) {
+        qpos = pos;
+        m = kNone;
+        l = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; db++) {
+            o[db] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (split) ol[db] = o[db];
+        }
+    }
+
+    // q from the row at p (global memory or LDS), 16-byte aligned if vec
+    __device__ void load(const typename PagedType<TYPE>::Io* p, bool vec, int g16, float qscale) {
+        if constexpr (!split) {
+            cs = qscale;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if (vec) q[ks] = *(const V8*)(p + 32 * ks + 8 * g16);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; e++) q[ks][e] = p[32 * ks + 8 * g16 + e];
+            }
+        } else {
+            float x[KS][8], mx = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float4 y = load4(p + 32 * ks + 8 * g16 + 4 * h, vec);
+                    x[ks][4 * h] = y.x;
+                    x[ks][4 * h + 1] = y.y;
+                    x[ks][4 * h + 2] = y.z;
+                    x[ks][4 * h + 3] = y.w;
+                }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[ks][e]));
+            mx = max_x32(max_x16(mx));
+            // 2^s with the largest element in [2^14, 2^15); 1 for zero and non-finite rows
+            const int be = (int)((__float_as_uint(mx) >> 23) & 0xFFu);
+            const int s = be == 0 || be == 255 ? 0 : min(141 - be, 126);
+            const float up = power2(s);
+            cs = qscale * power2(-s);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float y = x[ks][e] * up;
+                    q[ks][e] = (_Float16)y;
+                    ql[ks][e] = (_Float16)(y - (float)q[ks][e]);
+                }
+        }
+    }
+};
+
+// One tile of KEYS keys from key0 on for RB row blocks. kl and vl: the tile in LDS. masked:
+// some row of the wave ends inside the tile.
+template <int TYPE, int HD, int KEYS, int RB>
+__device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const char* kl, const char* vl, int key0, bool masked,
+                                          const int (&koff)[Geo<HD>::KS], const int (&voff)[Geo<HD>::DB], int g16) {
+    typedef Ops<TYPE> O;
+    typedef typename O::V8 V8;
+    typedef Geo<HD> G;
+    constexpr int KB = KEYS / 16;
+    floatx4 s[RB][KB];
+#pragma unroll
+    for (int r = 0; r < RB; r++)
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++) s[r][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ks++) {
+        V8 kf[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++) kf[kb] = *(const V8*)(kl + koff[ks] + kb * G::BLKB);
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) s[r][kb] = O::mul(kf[kb], rb[r].q[ks], s[r][kb]);
+        if constexpr (O::split) {
+#pragma unroll
+            for (int r = 0; r < RB; r++)
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) s[r][kb] = O::mul(kf[kb], rb[r].ql[ks], s[r][kb]);
+        }
+    }
+    // keys key0 + 16 kb + 4 g16 + e of row c16
+    V8 ph[RB][KB / 2], pl[O::split ? RB : 1][KB / 2];
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        RowBlock<TYPE, HD>& b = rb[r];
+        if (masked) {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (key0 + 16 * kb + 4 * g16 + e > b.qpos) s[r][kb][e] = -__builtin_huge_valf();
+        }
+        float mx = s[r][0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[r][kb][e]);
+        mx = max_x32(max_x16(mx));
+        if (__any((mx - b.m) * b.cs > kSlack)) {
+            const float to = fmaxf(b.m, mx);
+            const float corr = fast_exp2((b.m - to) * b.cs);
+            b.m = to;
+            b.l *= corr;
+#pragma unroll
+            for (int db = 0; db < G::DB; db++) {
+                b.o[db] *= corr;
+                if constexpr (O::split) b.ol[db] *= corr;
+            }
+        }
+        // fp16's scale of P joins the exponent where half a step of fp16 hides its rounding
+        const float mc = O::split ? b.m * b.cs : b.m * b.cs - (O::scale > 1.0f ? 11.0f : 0.0f);
+        // k-step h: keys 4 g16 .. +3 of key block 2 h, then of block 2 h + 1
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float p = fast_exp2(fmaf(s[r][kb][e], b.cs, -mc));
+                if constexpr (O::split) p *= O::scale;
+                b.l += p;
+                ph[r][kb >> 1][4 * (kb & 1) + e] = (typename PagedType<TYPE>::Page)p;
+                if constexpr (O::split)
+                    pl[r][kb >> 1][4 * (kb & 1) + e] = (_Float16)((p - (float)ph[r][kb >> 1][4 * (kb & 1) + e]) * kLow);
+            }
+    }
+#pragma unroll
+    for (int h = 0; h < KB / 2; h++)
+#pragma unroll
+        for (int db = 0; db < G::DB; db++) {
+            short4v part[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                part[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4v*)(vl + voff[db] + (2 * h + t) * G::BLKB));
+            const short __attribute__((ext_vector_type(8))) both = {part[0][0], part[0][1], part[0][2], part[0][3],
+                                                                    part[1][0], part[1][1], part[1][2], part[1][3]};
+            const V8 vf = __builtin_bit_cast(V8, both);
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                rb[r].o[db] = O::mul(vf, ph[r][h], rb[r].o[db]);
+                if constexpr (O::split) rb[r].ol[db] = O::mul(vf, pl[r][h], rb[r].ol[db]);
+            }
+        }
+}
+
+// Up to four rows again, packed rows r0 .. r0 + 3 of which those in `bad`, over their keys of tiles
+// first, first + step, ... below end, in fp32 from q on. Row, maximum (log2 units) and sum of
+// each go to res (rows of QS floats), m_out and l_out in the scale of the tiles' results. Lane = key
+// for the scores, 64 keys at a time; lane = pair of dims for the sums over V. qs: room for
+// four rows of QS floats.
+template <int TYPE, int HD, int KEYS>
+__device__ __forceinline__ void slow_rows(const PagedAttn& a, const Column& c, float* qs, int r0, unsigned bad, int first,
+                                          int step, int end, int lane, float* res, float* m_out, float* l_out) {
+    typedef typename PagedType<TYPE>::Io Io;
+    typedef typename PagedType<TYPE>::Page Page;
+    constexpr int QS = Geo<HD>::QS, NP = (HD / 2 + 63) / 64;
+    constexpr int TPI = 64 / KEYS;  // tiles at a time
+    int qp[4], qlast = -1;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int R = min(r0 + r, c.rows - 1);
+        qp[r] = c.hist + R / a.g;
+        qlast = max(qlast, qp[r]);
+        const Io* p = (const Io*)a.q + row_offset<HD>(a, c, R, a.ldq);
+        for (int e = lane; e < HD; e += 64) qs[r * QS + e] = (float)p[e] * a.qscale;
+    }
+    wave_sync();
+    float m[4], l[4], acc[4][2 * NP];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        m[r] = kNone;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NP; i++) acc[r][i] = 0.0f;
+    }
+#pragma unroll 1
+    for (int kt = first; kt < end && kt * KEYS <= qlast; kt += TPI * step) {
+        const int tile = kt + lane / KEYS * step, key = tile * KEYS + lane % KEYS;
+        const bool in = tile < end && key <= qlast;
+        const int at = in ? key : kt * KEYS;  // some key that exists
+        const int pi = at >> a.shift;
+        const int page = a.pages[c.table + (c.list ? c.list[pi] : pi)];
+        // within a layer's rows, which fit 31 bits
+        const int krow = (int)((((unsigned)page * a.n_kv + c.kvh) << a.shift) + (at & ((1 << a.shift) - 1)));
+        const u32x4* kr = (const u32x4*)(a.kp + (size_t)krow * Geo<HD>::ROWB);
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int ch = 0; ch < HD / 8; ch++) {
+            const u32x4 u = kr[ch];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float* x = qs + r * QS + 8 * ch;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[r] = fmaf(x[2 * e], from_page<Page>((uint16_t)(u[e] & 0xFFFFu)), s[r]);
+                    s[r] = fmaf(x[2 * e + 1], from_page<Page>((uint16_t)(u[e] >> 16)), s[r]);
+                }
+            }
+        }
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const bool valid = in && key <= qp[r];
+            const float sv = valid ? s[r] : -__builtin_huge_valf();
+            const bool nan = __any(valid && !(s[r] == s[r]));
+            const float mn = nan ? __builtin_nanf("") : fmaxf(m[r], group_max<64>(sv));
+            const float corr = fast_exp2(m[r] - mn);
+            p[r] = valid ? fast_exp2(sv - mn) * Ops<TYPE>::scale : 0.0f;
+            l[r] = l[r] * corr + group_sum<64>(p[r]);
+            m[r] = mn;
+#pragma unroll
+            for (int i = 0; i < 2 * NP; i++) acc[r][i] *= corr;
+        }
+        for (int j0 = 0; j0 < 64; j0 += 8) {
+            uint32_t v[8][NP];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {  // past the last key: the row of a key that exists, with weight 0 left out below
+                const int vrow = __builtin_amdgcn_readlane(krow, j0 + u);
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const int d = 2 * (lane + 64 * i);
+                    v[u][i] = d < HD ? *(const uint32_t*)(a.vp + (size_t)vrow * Geo<HD>::ROWB + 2 * d) : 0u;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int tj = kt + (j0 + u) / KEYS * step, kj = tj * KEYS + (j0 + u) % KEYS;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (tj >= end || kj > qp[r]) continue;
+                    const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p[r]), j0 + u));
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        acc[r][2 * i] = fmaf(pj, from_page<Page>((uint16_t)(v[u][i] & 0xFFFFu)), acc[r][2 * i]);
+                        acc[r][2 * i + 1] = fmaf(pj, from_page<Page>((uint16_t)(v[u][i] >> 16)), acc[r][2 * i + 1]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (!((bad >> r) & 1u)) continue;
+#pragma unroll
+        for (int i = 0; i < NP; i++)
+            if (2 * (lane + 64 * i) < HD) *(float2*)(res + r * QS + 2 * (lane + 64 * i)) = float2{acc[r][2 * i], acc[r][2 * i + 1]};
+        if (lane == 0) {
+            m_out[r] = m[r];
+            l_out[r] = l[r];
+        }
+    }
+    wave_sync();
+}
+
+// A wave's row block to LDS: rows of QS floats at res, maximum (log2 units) and sum; rows that are
+// not finite computed again over tiles first, first + step, ... below end.
+template <int TYPE, int HD, int KEYS>
+__device__ __forceinline__ void finish_rows(const PagedAttn& a, const Column& c, RowBlock<TYPE, HD>& b, int R0, int first,
+                                            int step, int end, int lane, float* res, float* qs, float* m_out, float* l_out) {
+    constexpr int DB = Geo<HD>::DB, QS = Geo<HD>::QS;
+    const int c16 = lane & 15, g16 = lane >> 4;
+    const float l = sum_x32(sum_x16(b.l));
+    float chk = l * 0.0f;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (Ops<TYPE>::split) b.o[db][e] = fmaf(b.ol[db][e], 1.0f / kLow, b.o[db][e]);
+            chk = fmaf(b.o[db][e], 0.0f, chk);
+        }
+    const bool sees = first < end && first * KEYS <= b.qpos;  // a key of these tiles
+    const bool good = chk == 0.0f && (l > 0.0f || !sees);
+    const unsigned long long lanes = __ballot(!good && R0 + c16 < c.rows);
+    const unsigned bad = (unsigned)((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xFFFFu);
+#pragma unroll
+    for (int db = 0; db < DB; db++) *(floatx4*)(res + c16 * QS + 16 * db + 4 * g16) = b.o[db];
+    if (g16 == 0) {
+        m_out[c16] = b.m > kNone ? b.m * b.cs : kNone;
+        l_out[c16] = l;
+    }
+    wave_sync();
+    if (bad) {
+#pragma unroll 1
+        for (int r = 0; r < 16; r += 4)
+            if ((bad >> r) & 15u)
+                slow_rows<TYPE, HD, KEYS>(a, c, qs, R0 + r, bad >> r, first, step, end, lane, res + r * QS, m_out + r, l_out + r);
+    }
+}
+
+// One output row's four elements: x / l, or 0 / 0 as the formula has it where every score is -inf.
+template <int TYPE, int HD>
+__device__ __forceinline__ void store_out(const PagedAttn& a, const Column& c, int R, int d, floatx4 x, float l) {
+    typedef typename PagedType<TYPE>::Io Io;
+    const float inv = 1.0f / l;
+    Io* p = (Io*)a.out + row_offset<HD>(a, c, R, a.ldo) + d;
+    store4(p, l == 0.0f ? float4{x[0] / l, x[1] / l, x[2] / l, x[3] / l} : float4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv},
+           a.ovec);
+}
+
+// The parts of rows [r0, r0 + ROWS): part p at slot slot0 + p, rows of HD floats, then ROWS
+// maxima and ROWS sums.
+template <int HD, int ROWS>
+struct Slots {
+    static constexpr size_t FLOATS = (size_t)ROWS * (HD + 2);
+};
+
+// Called by the whole workgroup after its part's stores; true in the workgroup that finishes
+// last, which then sees all parts. Its counter is zero again for the next call.
+__device__ __forceinline__ bool last_of(unsigned* counter, int parts, int* flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores are in its die's L2
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");  // and from there visible to the other dies
+        const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = n == (unsigned)parts - 1;
+        if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*flag) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return true;
+}
+
+template <int TYPE, int HD, int ROWS>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const Column& c, int slot0, int parts, int rows) {
+    constexpr int D4 = HD / 4;
+    constexpr size_t F = Slots<HD, ROWS>::FLOATS;
+    const float* base = a.part + (size_t)slot0 * F;
+    for (int it = threadIdx.x; it < rows * D4; it += blockDim.x) {
+        const int r = it / D4, d = 4 * (it - r * D4);
+        float M = kNone, L = 0.0f;
+        bool nan = false;
+#pragma unroll 4
+        for (int p = 0; p < parts; p++) {
+            const float m = base[p * F + ROWS * HD + r];
+            nan |= !(m == m);
+            M = fmaxf(M, m);
+        }
+        if (nan) M = __builtin_nanf("");
+        floatx4 A = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int p = 0; p < parts; p++) {
+            const float* s = base + p * F;
+            const float w = fast_exp2(s[ROWS * HD + r] - M);
+            L = fmaf(w, s[ROWS * HD + ROWS + r], L);
+            A += w * *(const floatx4*)(s + r * HD + d);
+        }
+        store_out<TYPE, HD>(a, c, c.r0 + r, d, A, L);
+    }
+}
+
+// Parts of a column over chosen pages: as many as leave no workgroup idle, each with a tile per wave.
+__host__ __device__ inline int chosen_parts(int wgs, int cols, int select, int shift) {
+    if (cols <= 0) return 1;
+    const long long keys = (long long)select << shift, piece = kNarrowKeys * kNarrowLeast;
+    const long long most = (keys + piece - 1) / piece, room = wgs / cols;
+    return (int)(room < 1 ? 1 : room < most ? room : most);
+}
+
+template <int HD>
+constexpr int narrow_waves() { return HD <= 128 ? 4 : 2; }
+
+// ---- up to 16 rows: waves on different key tiles ----
+template <int TYPE, int HD>
+__global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
+    typedef Geo<HD> G;
+    typedef typename PagedType<TYPE>::Io Io;
+    constexpr int KW = narrow_waves<HD>(), KEYS = kNarrowKeys, KB = KEYS / 16;
+    constexpr int LPW = 2 * KB * G::PPB;  // loads per tile
+    constexpr int QB = HD * (int)sizeof(Io), QP = 16 * QB / 1024;  // bytes of a q row, 1 KB loads of 16 of them
+    constexpr int D4 = HD / 4;
+    __shared__ __attribute__((aligned(1024))) char lds[KW][2][2][KB * G::BLKB];  // [wave][buffer][K, V]
+    __shared__ __attribute__((aligned(1024))) char sq[16 * QB];
+    __shared__ float s_ml[KW][2][16];
+    __shared__ int s_flag;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g16 = lane >> 4;
+
+    // lane offsets of a block's loads and of the operands in a tile
+    unsigned goff[2][G::PPB];
+#pragma unroll
+    for (int i = 0; i < G::PPB; i++) {
+        const int L = 64 * i + lane, r = L / G::CH, ch = L % G::CH;
+        goff[0][i] = r * G::ROWB + 16 * (ch ^ G::xk(r));
+        goff[1][i] = r * G::ROWB + 16 * (ch ^ G::xv(r));
+    }
+    int koff[G::KS], voff[G::DB];
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ks++) koff[ks] = c16 * G::ROWB + 16 * ((4 * ks + g16) ^ G::xk(c16));
+    const int vr0 = 4 * g16 + (c16 >> 2);
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+        voff[db] = vr0 * G::ROWB + 16 * ((2 * db + ((c16 & 3) >> 1)) ^ G::xv(vr0)) + 8 * (c16 & 1);
+
+    // the work: a run of the plan's items, or (chosen pages) columns of one token, KV head and 16
+    // of its heads, each in as many parts as leave no workgroup idle
+    const int n_blk = (a.g + 15) / 16;
+    int it, it_end, it_step, parts = 1, cols = 0;
+    if (a.chosen) {
+        cols = scalar_int(a.header, kHdTokens) * a.n_kv * n_blk;
+        parts = chosen_parts(a.wgs, cols, a.select, a.shift);
+        it = blockIdx.x;
+        it_end = cols * parts;
+        it_step = gridDim.x;
+    } else {
+        it = scalar_int(a.first, blockIdx.x);
+        it_end = scalar_int(a.first, blockIdx.x + 1);
+        it_step = 1;
+    }
+    for (; it < it_end; it += it_step) {
+        Column c;
+        int t0, t1, slot0, part, counter;
+        if (a.chosen) {
+            const int col = it / parts;
+            part = it - col * parts;
+            const int blk = col % n_blk, tk = col / n_blk, tok = tk / a.n_kv;
+            const int sq4 = 4 * scalar_int(a.token_seq, tok);
+            const int row0 = scalar_int(a.seqs, sq4), n_new = scalar_int(a.seqs, sq4 + 1), len = scalar_int(a.seqs, sq4 + 2);
+            const int pos = len - n_new + tok - row0;
+            const int seen = min(a.select, (pos >> a.shift) + 1);  // pages, the last of them the token's own
+            c.kend = ((seen - 1) << a.shift) + (pos & ((1 << a.shift) - 1)) + 1;
+            c.row0 = tok;
+            c.rows = a.g;
+            c.hist = c.kend - 1;
+            c.table = scalar_int(a.seqs, sq4 + 3);
+            c.kvh = tk - tok * a.n_kv;
+            c.r0 = 16 * blk;
+            c.list = a.chosen + (size_t)tk * a.select;
+            const int tiles = (c.kend + KEYS - 1) / KEYS;
+            t0 = (int)((long long)tiles * part / parts);
+            t1 = (int)((long long)tiles * (part + 1) / parts);
+            slot0 = col * parts;
+            counter = col;
+        } else {
+            const int* p = a.items + (size_t)it * (sizeof(PagedItem) / 4);
+            c.row0 = scalar_int(p, 0);
+            c.rows = scalar_int(p, 1);
+            c.hist = scalar_int(p, 2);
+            c.table = scalar_int(p, 3);
+            c.kvh = scalar_int(p, 4);
+            c.r0 = scalar_int(p, 5);
+            t0 = scalar_int(p, 6);
+            t1 = scalar_int(p, 7);
+            slot0 = scalar_int(p, 8);
+            part = scalar_int(p, 9);
+            parts = scalar_int(p, 10);
+            counter = scalar_int(p, 11);
+            c.kend = c.hist + (c.rows - 1) / a.g + 1;
+            c.list = nullptr;
+        }
+        const int nrow = min(16, c.rows - c.r0);
+        const int tile0 = t0 + w;  // this wave's tiles: tile0, tile0 + KW, ...
+
+        int page[KB];  // of the tile that is loaded next
+        auto look = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < KB; b++) page[b] = page_at(a, c, min(kt * KEYS + 16 * b, c.kend - 1) >> a.shift);
+        };
+        auto issue = [&](int kt, int buf) __attribute__((always_inline)) {
+            if (kt >= t1) return;
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                const int pos = min(kt * KEYS + 16 * b, (c.kend - 1) & ~15);  // a block past the last one: that one again
+                const size_t at = block_offset<HD>(a, c, page[b], pos);
+                const int last = c.kend - 1 - pos;  // rows past the last key repeat it (and are masked)
+#pragma unroll
+                for (int o = 0; o < 2; o++) {
+                    const char* src = (o ? a.vp : a.kp) + at;
+#pragma unroll
+                    for (int i = 0; i < G::PPB; i++) {
+                        unsigned off = goff[o][i];
+                        if (last < 15) {
+                            const int L = 64 * i + lane, r = L / G::CH;
+                            off = min(r, last) * G::ROWB + 16 * ((L % G::CH) ^ (o ? G::xv(r) : G::xk(r)));
+                        }
+                        lds_dma_b128(src, off, lds_addr(&lds[w][buf][o][b * G::BLKB + 1024 * i]));
+                    }
+                }
+            }
+            if (kt + KW < t1) look(kt + KW);
+        };
+        if (tile0 < t1) look(tile0);
+        // q ahead of the tiles, so that the wave can wait for it alone
+        const Io* q = (const Io*)a.q;
+        if (a.qvec) {
+            for (int i = w; i < QP; i += KW) {
+                const int L = 64 * i + lane, r = L / (QB / 16);
+                const char* p = (const char*)(q + row_offset<HD>(a, c, c.r0 + min(r, nrow - 1), a.ldq)) + 16 * (L % (QB / 16));
+                lds_dma_b128_at(p, lds_addr(sq + 1024 * i));
+            }
+        } else {
+            for (int i = tid; i < 16 * HD; i += 64 * KW) {
+                const int r = i / HD;
+                ((Io*)sq)[i] = q[row_offset<HD>(a, c, c.r0 + min(r, nrow - 1), a.ldq) + i - r * HD];
+            }
+        }
+        issue(tile0, 0);
+        issue(tile0 + KW, 1);
+        const int mine = tile0 >= t1 ? 0 : tile0 + KW >= t1 ? 1 : 2;
+        if (mine == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPW < 63 ? 2 * LPW : 63) : "memory");
+        else if (mine == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPW < 63 ? LPW : 63) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        RowBlock<TYPE, HD> rb[1];
+        rb[0].load((const Io*)sq + c16 * HD, true, g16, a.qscale);
+        rb[0].start(c.hist + min(c.r0 + c16, c.rows - 1) / a.g);
+        const int qmin = c.hist + c.r0 / a.g;
+
+        int buf = 0;
+        for (int kt = tile0; kt < t1; kt += KW) {
+            if (kt + KW < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPW < 63 ? LPW : 63) : "memory");  // the next tile's stay in flight
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            tile_step<TYPE, HD, KEYS, 1>(rb, lds[w][buf][0], lds[w][buf][1], kt * KEYS, kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer has been read
+            issue(kt + 2 * KW, buf);
+            buf ^= 1;
+        }
+
+        // the waves' results to their own tile buffers, then together
+        float* res = (float*)&lds[w][0][0][0];
+        finish_rows<TYPE, HD, KEYS>(a, c, rb[0], c.r0, tile0, KW, t1, lane, res, res + 16 * G::QS, s_ml[w][0], s_ml[w][1]);
+        __syncthreads();
+        float* slot = a.part + (size_t)(slot0 + part) * Slots<HD, 16>::FLOATS;
+        for (int i = tid; i < nrow * D4; i += 64 * KW) {
+            const int r = i / D4, d = 4 * (i - r * D4);
+            float M = kNone, L = 0.0f;
+            bool nan = false;
+            floatx4 A = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KW; k++) {
+                const float m = s_ml[k][0][r];
+                nan |= !(m == m);
+                M = fmaxf(M, m);
+            }
+            if (nan) M = __builtin_nanf("");
+#pragma unroll
+            for (int k = 0; k < KW; k++) {
+                const float e = fast_exp2(s_ml[k][0][r] - M);
+                L = fmaf(e, s_ml[k][1][r], L);
+                A += e * *(const floatx4*)((const float*)&lds[k][0][0][0] + r * G::QS + d);
+            }
+            if (parts > 1) {
+                *(floatx4*)(slot + r * HD + d) = A;
+                if (d == 0) {
+                    slot[16 * HD + r] = M;
+                    slot[16 * HD + 16 + r] = L;
+                }
+            } else {
+                store_out<TYPE, HD>(a, c, c.r0 + r, d, A, L);
+            }
+        }
+        if (parts > 1 && last_of(a.counters + counter, parts, &s_flag)) join_parts<TYPE, HD, 16>(a, c, slot0, parts, nrow);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no store among the next item's counted loads
+        __syncthreads();  // LDS is free again
+    }
+}
+
+template <int TYPE, int HD>
+constexpr int wide_blocks() { return TYPE != PQA_PAGED_F32 && HD <= 128 ? 2 : 1; }
+template <int HD>
+constexpr int wide_keys() { return HD > 192 ? 32 : 64; }
+
+// ---- more rows: 4 waves share each key tile, RB blocks of 16 rows each ----
+template <int TYPE, int HD>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_wide_kernel(const PagedAttn a) {
+    typedef Geo<HD> G;
+    typedef typename PagedType<TYPE>::Io Io;
+    constexpr int KEYS = wide_keys<HD>(), KB = KEYS / 16, RB = wide_blocks<TYPE, HD>(), ROWS = 64 * RB;
+    constexpr int D4 = HD / 4;
+    constexpr int TILE = KB * G::BLKB;
+    constexpr int WAVE = 20 * G::QS * 4;  // a wave's result and its slow rows' q
+    constexpr int BYTES = 4 * TILE > 4 * WAVE ? 4 * TILE : 4 * WAVE;
+    __shared__ __attribute__((aligned(1024))) char lds[BYTES];  // [buffer][K, V][TILE]
+    __shared__ float s_ml[4][2][16];
+    __shared__ int s_flag;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g16 = lane >> 4;
+    // the wave's share of a tile's loads: block lb of 16 keys, operands lo0 .. lo1
+    constexpr int OPS = KB == 4 ? 2 : 1;
+    const int lb = w & (KB - 1), lo0 = KB == 4 ? 0 : w >> 1;
+    int koff[G::KS], voff[G::DB];
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ks++) koff[ks] = c16 * G::ROWB + 16 * ((4 * ks + g16) ^ G::xk(c16));
+    const int vr0 = 4 * g16 + (c16 >> 2);
+#pragma unroll
+    for (int db = 0; db < G::DB; db++)
+        voff[db] = vr0 * G::ROWB + 16 * ((2 * db + ((c16 & 3) >> 1)) ^ G::xv(vr0)) + 8 * (c16 & 1);
+    unsigned goff[OPS][G::PPB];
+#pragma unroll
+    for (int o = 0; o < OPS; o++)
+#pragma unroll
+        for (int i = 0; i < G::PPB; i++) {
+            const int L = 64 * i + lane, r = L / G::CH;
+            goff[o][i] = r * G::ROWB + 16 * ((L % G::CH) ^ (lo0 + o ? G::xv(r) : G::xk(r)));
+        }
+
+    const int n_items = scalar_int(a.header, kHdWide);
+    for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+        const int* p = a.items + (size_t)it * (sizeof(PagedItem) / 4);
+        Column c;
+        c.row0 = scalar_int(p, 0);
+        c.rows = scalar_int(p, 1);
+        c.hist = scalar_int(p, 2);
+        c.table = scalar_int(p, 3);
+        c.kvh = scalar_int(p, 4);
+        c.r0 = scalar_int(p, 5);
+        const int t0 = scalar_int(p, 6), t1 = scalar_int(p, 7), slot0 = scalar_int(p, 8), part = scalar_int(p, 9),
+                  parts = scalar_int(p, 10), counter = scalar_int(p, 11);
+        c.kend = c.hist + (c.rows - 1) / a.g + 1;
+        c.list = nullptr;
+
+        int page;  // of the wave's block in the tile that is loaded next
+        auto look = [&](int kt) __attribute__((always_inline)) {
+            page = page_at(a, c, min(kt * KEYS + 16 * lb, c.kend - 1) >> a.shift);
+        };
+        auto issue = [&](int kt, int buf) __attribute__((always_inline)) {
+            if (kt >= t1) return;
+            const int pos = min(kt * KEYS + 16 * lb, (c.kend - 1) & ~15);
+            const size_t at = block_offset<HD>(a, c, page, pos);
+            const int last = c.kend - 1 - pos;
+#pragma unroll
+            for (int o = 0; o < OPS; o++) {
+                const char* src = (lo0 + o ? a.vp : a.kp) + at;
+#pragma unroll
+                for (int i = 0; i < G::PPB; i++) {
+                    unsigned off = goff[o][i];
+                    if (last < 15) {
+                        const int L = 64 * i + lane, r = L / G::CH;
+                        off = min(r, last) * G::ROWB + 16 * ((L % G::CH) ^ (lo0 + o ? G::xv(r) : G::xk(r)));
+                    }
+                    lds_dma_b128(src, off, lds_addr(lds + (2 * buf + lo0 + o) * TILE + lb * G::BLKB + 1024 * i));
+                }
+            }
+            if (kt + 1 < t1) look(kt + 1);
+        };
+        const int R0 = c.r0 + 16 * RB * w;  // the wave's rows
+        RowBlock<TYPE, HD> rb[RB];
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            const int R = min(R0 + 16 * r + c16, c.rows - 1);
+            rb[r].load((const Io*)a.q + row_offset<HD>(a, c, R, a.ldq), a.qvec, g16, a.qscale);
+            rb[r].start(c.hist + R / a.g);
+        }
+        const int qmin = c.hist + min(R0, c.rows - 1) / a.g;
+        const int qmax = R0 < c.rows ? c.hist + min(R0 + 16 * RB - 1, c.rows - 1) / a.g : -1;
+        look(t0);
+        issue(t0, 0);
+        int buf = 0;
+        for (int kt = t0; kt < t1; kt++) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the tile
+            __syncthreads();                                   // everyone's; the other buffer is free
+            issue(kt + 1, buf ^ 1);
+            if (kt * KEYS <= qmax)
+                tile_step<TYPE, HD, KEYS, RB>(rb, lds + 2 * buf * TILE, lds + (2 * buf + 1) * TILE, kt * KEYS,
+                                              kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
+            buf ^= 1;
+        }
+        __syncthreads();  // the tiles have been read
+        float* res = (float*)(lds + w * WAVE);
+        float* slot = a.part + (size_t)(slot0 + part) * Slots<HD, ROWS>::FLOATS;
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            const int first = R0 + 16 * r, n = min(16, c.rows - first);
+            if (n <= 0) break;
+            finish_rows<TYPE, HD, KEYS>(a, c, rb[r], first, t0, 1, t1, lane, res, res + 16 * G::QS, s_ml[w][0], s_ml[w][1]);
+            for (int i = lane; i < n * D4; i += 64) {
+                const int j = i / D4, d = 4 * (i - j * D4), at = 16 * (RB * w + r) + j;
+                const floatx4 x = *(const floatx4*)(res + j * G::QS + d);
+                if (parts > 1) {
+                    *(floatx4*)(slot + at * HD + d) = x;
+                    if (d == 0) {
+                        slot[ROWS * HD + at] = s_ml[w][0][j];
+                        slot[ROWS * HD + ROWS + at] = s_ml[w][1][j];
+                    }
+                } else {
+                    store_out<TYPE, HD>(a, c, first + j, d, x, s_ml[w][1][j]);
+                }
+            }
+            wave_sync();
+        }
+        if (parts > 1 && last_of(a.counters + counter, parts, &s_flag))
+            join_parts<TYPE, HD, ROWS>(a, c, slot0, parts, min(ROWS, c.rows - c.r0));
+        __syncthreads();  // LDS is free again
+    }
+}
+
+template <int TYPE, int HD>
+hipError_t launch_kernels(const PagedAttn& a, PagedAttn wide, int narrow_grid, int wide_grid, hipStream_t s) {
+    if (narrow_grid) {
+        hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD>), dim3((unsigned)narrow_grid), dim3(64 * narrow_waves<HD>()), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (wide_grid) {
+        hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+template <int TYPE>
+hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, int narrow_grid, int wide_grid, hipStream_t s) {
+    switch (hd) {
+#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, narrow_grid, wide_grid, s);
+        PQA_PG(64) PQA_PG(96) PQA_PG(128) PQA_PG(160) PQA_PG(192) PQA_PG(256)
+#undef PQA_PG
+        default: return hipErrorInvalidValue;
+    }
+}
+
+hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, int narrow_grid, int wide_grid, hipStream_t s) {
+    switch (b->p->type) {
+        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
+        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
+    }
+}
+
+PagedAttn arguments(const pqa_batch* b, int layer, const PagedRows& q, void* out, long long ldo) {
+    const pqa_paged* p = b->p;
+    const size_t io = (size_t)paged_io_bytes(p->type);
+    PagedAttn a{};
+    a.q = q.p;
+    a.out = out;
+    a.ldq = q.ld;
+    a.ldo = ldo;
+    a.kp = p->k + (size_t)layer * p->layer_bytes;
+    a.vp = p->v + (size_t)layer * p->layer_bytes;
+    a.pages = b->pages;
+    a.items = (const int*)b->narrow;
+    a.first = b->narrow_first;
+    a.header = b->header;
+    a.part = b->part_narrow;
+    a.counters = b->counters;
+    a.token_seq = b->token_seq;
+    a.seqs = (const int*)b->seqs;
+    a.wgs = b->shape.narrow_wgs;
+    a.g = p->group;
+    a.n_kv = p->n_kv;
+    a.shift = p->page_shift;
+    a.qvec = ((uintptr_t)q.p & 15) == 0 && q.ld * io % 16 == 0;
+    a.ovec = ((uintptr_t)out & (4 * io - 1)) == 0 && ldo % 4 == 0;
+    a.qscale = 1.4426950408889634f / sqrtf((float)p->head_dim);
+    return a;
+}
+
+}  // namespace
+
+int paged_wide_rows(int type, int hd) { return type != PQA_PAGED_F32 && hd <= 128 ? 128 : 64; }
+int paged_wide_keys(int hd) { return hd > 192 ? 32 : 64; }
+int paged_narrow_wgs(int hd, int cu_count) { return hd == 64 ? 2 * cu_count : cu_count; }
+int paged_wide_wgs(int hd, int cu_count) { return hd <= 128 ? 2 * cu_count : cu_count; }
+
+hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q, void* out, long long ldo, bool captured,
+                               hipStream_t s) {
+    const PagedAttn a = arguments(b, layer, q, out, ldo);
+    PagedAttn wide = a;
+    wide.items = (const int*)b->wide;
+    wide.part = b->part_wide;
+    wide.counters = b->counters + b->shape.narrow_wgs;
+    // A captured call may be replayed with what the batch holds then: both kernels, on grids that
+    // any content fits
+    const int n = captured ? b->shape.narrow_wgs : b->plan.narrow_active;
+    const int w = captured ? b->shape.wide_wgs : (int)b->plan.wide.size();
+    return launch_any(b, a, wide, n, w, s);
+}
+
+hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q, int select, const int* chosen, void* out,
+                               long long ldo, bool captured, hipStream_t s) {
+    PagedAttn a = arguments(b, layer, q, out, ldo);
+    a.chosen = chosen;
+    a.select = select;
+    const long long cols = (long long)b->plan.n_tok * b->p->n_kv * ((b->p->group + 15) / 16);
+    const long long grid = captured ? b->shape.narrow_wgs : cols * chosen_parts(a.wgs, (int)cols, select, a.shift);
+    return launch_any(b, a, a, (int)std::min<long long>(grid, 1 << 30), 0, s);
+}
+
+}  // namespace pqa
