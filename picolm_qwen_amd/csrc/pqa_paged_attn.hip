@@ -440,55 +440,107 @@ __device__ __forceinline__ void store_out(const PagedAttn& a, const Column& c, i
            a.ovec);
 }
 
-// The parts of rows [r0, r0 + ROWS): part p at slot slot0 + p, rows of HD floats, then ROWS
-// maxima and ROWS sums.
+// The parts of rows [r0, r0 + ROWS): part p at slot slot0 + p, rows of HD floats, then a
+// maximum and a sum per row.
 template <int HD, int ROWS>
 struct Slots {
     static constexpr size_t FLOATS = (size_t)ROWS * (HD + 2);
 };
 
+// Partial results pass between workgroups on different dies, whose L2s are not coherent: stored
+// and loaded past them (agent scope, relaxed), so that no cache has to be written back or emptied.
+// (With a release and an acquire fence around plain accesses, which write back and empty an L2 per part,
+// a token of 32 / 8 heads of 128 at 2048 keys took 18.1 us; so 10.9.)
+__device__ __forceinline__ void part_store4(float* p, floatx4 x) {
+    const auto u = __builtin_bit_cast(unsigned long long __attribute__((ext_vector_type(2))), x);
+    __hip_atomic_store((unsigned long long*)p, (unsigned long long)u[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((unsigned long long*)p + 1, (unsigned long long)u[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ floatx4 part_load4(const float* p) {
+    unsigned long long __attribute__((ext_vector_type(2))) u;
+    u[0] = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    u[1] = __hip_atomic_load((const unsigned long long*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return __builtin_bit_cast(floatx4, u);
+}
+// a row's maximum and sum
+__device__ __forceinline__ void part_store2(float* p, float m, float l) {
+    __hip_atomic_store((unsigned long long*)p, (unsigned long long)__float_as_uint(l) << 32 | __float_as_uint(m), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 part_load2(const float* p) {
+    const unsigned long long u = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((unsigned)u), __uint_as_float((unsigned)(u >> 32))};
+}
+
 // Called by the whole workgroup after its part's stores; true in the workgroup that finishes
 // last, which then sees all parts. Its counter is zero again for the next call.
 __device__ __forceinline__ bool last_of(unsigned* counter, int parts, int* flag) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores are in its die's L2
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have reached memory
     __syncthreads();
     if (threadIdx.x == 0) {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");  // and from there visible to the other dies
         const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = n == (unsigned)parts - 1;
         if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!*flag) return false;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    return true;
+    asm volatile("" ::: "memory");  // the loads of the parts stay behind the counter
+    return *flag != 0;
 }
 
-template <int TYPE, int HD, int ROWS>
-__device__ __forceinline__ void join_parts(const PagedAttn& a, const Column& c, int slot0, int parts, int rows) {
+// Joins the parts of `rows` rows in the order of the parts. lds: BYTES of the workgroup's LDS; the
+// rows go in groups whose maxima and sums fit it. Where a group has fewer elements
+// than the workgroup threads, several threads share an element's parts.
+template <int TYPE, int HD, int ROWS, int BYTES>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const Column& c, int slot0, int parts, int rows, char* lds) {
     constexpr int D4 = HD / 4;
     constexpr size_t F = Slots<HD, ROWS>::FLOATS;
     const float* base = a.part + (size_t)slot0 * F;
-    for (int it = threadIdx.x; it < rows * D4; it += blockDim.x) {
-        const int r = it / D4, d = 4 * (it - r * D4);
-        float M = kNone, L = 0.0f;
-        bool nan = false;
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) {
-            const float m = base[p * F + ROWS * HD + r];
-            nan |= !(m == m);
-            M = fmaxf(M, m);
+    const int tid = threadIdx.x, nt = blockDim.x;
+    floatx4* s_a = (floatx4*)lds;                 // [threads]
+    float2* s_w = (float2*)(lds + 16 * 256);      // [rows of a group][parts]: weight and sum
+    const int fit = (BYTES - 16 * 256) / (8 * parts), step = min(rows, max(1, fit));
+    for (int g0 = 0; g0 < rows; g0 += step) {
+        const int n = min(step, rows - g0);
+        for (int i = tid; i < n * parts; i += nt) {
+            const int p = i / n, r = i - p * n;
+            s_w[r * parts + p] = part_load2(base + p * F + ROWS * HD + 2 * (g0 + r));
         }
-        if (nan) M = __builtin_nanf("");
-        floatx4 A = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) {
-            const float* s = base + p * F;
-            const float w = fast_exp2(s[ROWS * HD + r] - M);
-            L = fmaf(w, s[ROWS * HD + ROWS + r], L);
-            A += w * *(const floatx4*)(s + r * HD + d);
+        __syncthreads();
+        const int tasks = n * D4, share = max(1, min(parts, nt / tasks));
+        for (int i0 = 0; i0 < tasks * share; i0 += nt) {
+            const int i = i0 + tid, j = i / tasks, t = i - j * tasks, r = t / D4, d = 4 * (t - r * D4);
+            const bool live = i < tasks * share;
+            float M = kNone, L = 0.0f;
+            floatx4 A = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (live) {
+                const float2* w = s_w + r * parts;
+                bool nan = false;
+                for (int p = 0; p < parts; p++) {
+                    nan |= !(w[p].x == w[p].x);
+                    M = fmaxf(M, w[p].x);
+                }
+                if (nan) M = __builtin_nanf("");
+                for (int p = 0; p < parts; p++) L = fmaf(fast_exp2(w[p].x - M), w[p].y, L);
+                const float* src = base + (g0 + r) * HD + d;
+                int p = j;
+                for (; p + 7 * share < parts; p += 8 * share) {
+                    floatx4 x[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) x[u] = part_load4(src + (p + u * share) * F);
+#pragma unroll
+                    for (int u = 0; u < 8; u++) A += fast_exp2(w[p + u * share].x - M) * x[u];
+                }
+                for (; p < parts; p += share) A += fast_exp2(w[p].x - M) * part_load4(src + p * F);
+            }
+            if (share > 1) {  // then tasks * share <= threads: one turn
+                s_a[tid] = A;
+                __syncthreads();
+                if (live && j == 0)
+                    for (int u = 1; u < share; u++) A += s_a[tid + u * tasks];
+            }
+            if (live && j == 0) store_out<TYPE, HD>(a, c, c.r0 + g0 + r, d, A, L);
         }
-        store_out<TYPE, HD>(a, c, c.r0 + r, d, A, L);
+        __syncthreads();
     }
 }
 
@@ -685,16 +737,14 @@ __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void pag
                 A += e * *(const floatx4*)((const float*)&lds[k][0][0][0] + r * G::QS + d);
             }
             if (parts > 1) {
-                *(floatx4*)(slot + r * HD + d) = A;
-                if (d == 0) {
-                    slot[16 * HD + r] = M;
-                    slot[16 * HD + 16 + r] = L;
-                }
+                part_store4(slot + r * HD + d, A);
+                if (d == 0) part_store2(slot + 16 * HD + 2 * r, M, L);
             } else {
                 store_out<TYPE, HD>(a, c, c.r0 + r, d, A, L);
             }
         }
-        if (parts > 1 && last_of(a.counters + counter, parts, &s_flag)) join_parts<TYPE, HD, 16>(a, c, slot0, parts, nrow);
+        if (parts > 1 && last_of(a.counters + counter, parts, &s_flag)) 
+            join_parts<TYPE, HD, 16, (int)sizeof lds>(a, c, slot0, parts, nrow, &lds[0][0][0][0]);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no store among the next item's counted loads
         __syncthreads();  // LDS is free again
     }
@@ -814,11 +864,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_wide_kernel(cons
                 const int j = i / D4, d = 4 * (i - j * D4), at = 16 * (RB * w + r) + j;
                 const floatx4 x = *(const floatx4*)(res + j * G::QS + d);
                 if (parts > 1) {
-                    *(floatx4*)(slot + at * HD + d) = x;
-                    if (d == 0) {
-                        slot[ROWS * HD + at] = s_ml[w][0][j];
-                        slot[ROWS * HD + ROWS + at] = s_ml[w][1][j];
-                    }
+                    part_store4(slot + at * HD + d, x);
+                    if (d == 0) part_store2(slot + ROWS * HD + 2 * at, s_ml[w][0][j], s_ml[w][1][j]);
                 } else {
                     store_out<TYPE, HD>(a, c, first + j, d, x, s_ml[w][1][j]);
                 }
@@ -826,7 +873,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_wide_kernel(cons
             wave_sync();
         }
         if (parts > 1 && last_of(a.counters + counter, parts, &s_flag))
-            join_parts<TYPE, HD, ROWS>(a, c, slot0, parts, min(ROWS, c.rows - c.r0));
+            join_parts<TYPE, HD, ROWS, BYTES>(a, c, slot0, parts, min(ROWS, c.rows - c.r0), lds);
         __syncthreads();  // LDS is free again
     }
 }

@@ -175,7 +175,33 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
             cost += (long long)s.n_kv * ((q.len + kNarrowKeys - 1) / kNarrowKeys + kNarrowOverhead);
     int counter = 0;
     if (cost) {
-        const long long share = std::max<long long>((cost + s.narrow_wgs - 1) / s.narrow_wgs, kNarrowLeast + kNarrowOverhead);
+        // The least share that the workgroups can take all of: cuts cost more than the columns alone,
+        // so an even share of these is tried first and then grown.
+        long long share = std::max<long long>((cost + s.narrow_wgs - 1) / s.narrow_wgs, kNarrowLeast + kNarrowOverhead);
+        // what a workgroup takes of a column's `left` tiles with `room` to go; 0: nothing
+        auto piece = [](long long room, int left) {
+            const long long take = room - kNarrowOverhead;
+            return take < std::min(kNarrowLeast, left) ? 0 : left - take < kNarrowLeast ? left : (int)take;
+        };
+        for (;; share += share / 64 + 1) {
+            int need = 1;
+            long long room = share;
+            for (const PagedSeq& q : plan->seqs) {
+                if (!q.n_new || (long long)q.n_new * s.group > kNarrowRows) continue;
+                const int tiles = (q.len + kNarrowKeys - 1) / kNarrowKeys;
+                for (int kvh = 0; kvh < s.n_kv && need <= s.narrow_wgs; kvh++)
+                    for (int t = 0; t < tiles;) {
+                        const int take = piece(room, tiles - t);
+                        if (!take) {
+                            need++;
+                            room = share;
+                        }
+                        t += take;
+                        room -= take ? take + kNarrowOverhead : 0;
+                    }
+            }
+            if (need <= s.narrow_wgs) break;
+        }
         int w = 0, slot = 0;
         long long room = share;
         for (const PagedSeq& q : plan->seqs) {
@@ -183,18 +209,15 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
             const int tiles = (q.len + kNarrowKeys - 1) / kNarrowKeys;
             for (int kvh = 0; kvh < s.n_kv; kvh++) {
                 const size_t begin = plan->narrow.size();
-                int t = 0;
-                while (t < tiles) {
-                    // the last workgroup takes all that is left
-                    long long take = w == s.narrow_wgs - 1 ? tiles : room - kNarrowOverhead;
-                    if (take < std::min(kNarrowLeast, tiles - t)) {  // no room for a piece: the next workgroup
+                for (int t = 0; t < tiles;) {
+                    const int take = piece(room, tiles - t);
+                    if (!take) {  // no room for a piece: the next workgroup
                         plan->narrow_first[++w] = (int)plan->narrow.size();
                         room = share;
                         continue;
                     }
-                    if (tiles - t - take < kNarrowLeast) take = tiles - t;
-                    plan->narrow.push_back({q.row0, q.n_new * s.group, q.len - q.n_new, q.table, kvh, 0, t, (int)(t + take), 0, 0, 1, 0});
-                    t += (int)take;
+                    plan->narrow.push_back({q.row0, q.n_new * s.group, q.len - q.n_new, q.table, kvh, 0, t, t + take, 0, 0, 1, 0});
+                    t += take;
                     room -= take + kNarrowOverhead;
                 }
                 const int parts = (int)(plan->narrow.size() - begin);

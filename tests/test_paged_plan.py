@@ -129,6 +129,17 @@ int main() {
         for (int w = 0; w < s.narrow_wgs; w++) CHECK(p.narrow_first[w] <= p.narrow_first[w + 1]);
         CHECK(p.narrow_first[s.narrow_wgs] == (int)p.narrow.size());
         for (int w = p.narrow_active; w < s.narrow_wgs; w++) CHECK(p.narrow_first[w] == p.narrow_first[w + 1]);
+        {  // no workgroup has much more than its share of the tiles
+            long long tiles = 0, most = 0;
+            for (int w = 0; w < p.narrow_active; w++) {
+                long long mine = 0;
+                for (int i = p.narrow_first[w]; i < p.narrow_first[w + 1]; i++)
+                    mine += p.narrow[i].t1 - p.narrow[i].t0 + kNarrowOverhead;
+                tiles += mine;
+                most = std::max(most, mine);
+            }
+            CHECK(most <= tiles / s.narrow_wgs * 1.1 + 2 * (kNarrowOverhead + kNarrowLeast));
+        }
         if (check(trial, s, p, p.narrow, false) || check(trial, s, p, p.wide, true)) return 1;
         // what pqa_batch_create holds for the wide kernel's partials of this very batch
         size_t blocks = 0, cut = 0;
