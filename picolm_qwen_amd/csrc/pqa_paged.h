@@ -39,17 +39,16 @@ struct pqa_batch {
     // one device allocation: the tables below, then the partial results
     char* mem = nullptr;
     int* header = nullptr;  // kPagedHeader ints
-    pqa::PagedSeq* seqs = nullptr;
-    int* token_seq = nullptr;
+    pqa::PagedToken* tokens = nullptr;
     int* pages = nullptr;
     pqa::PagedTouched* touched = nullptr;
-    int* narrow_first = nullptr;
-    pqa::PagedItem* narrow = nullptr;
+    pqa::PagedRun* runs = nullptr;
+    pqa::PagedItem* rest = nullptr;
     pqa::PagedItem* wide = nullptr;
     unsigned* counters = nullptr;  // zero between calls: narrow_wgs, then wide_wgs
     float* part_narrow = nullptr;
     float* part_wide = nullptr;
-    size_t max_touched = 0, max_narrow = 0, max_wide = 0;
+    size_t max_touched = 0, max_rest = 0, max_wide = 0;
     // two pinned staging buffers in turn, so that a set waits for the copy before last
     char* stage[2] = {nullptr, nullptr};
     size_t stage_bytes[2] = {0, 0};
@@ -60,7 +59,7 @@ struct pqa_batch {
 namespace pqa {
 
 // what the kernels read of a batch, so that a captured call follows the batch's later sets
-enum : int { kHdTokens = 0, kHdTouched = 1, kHdWide = 2, kPagedHeader = 4 };
+enum : int { kHdTokens = 0, kHdTouched = 1, kHdRuns = 2, kHdWide = 3, kPagedHeader = 4 };
 
 inline bool paged_head_dim(int hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 160 || hd == 192 || hd == 256; }
 inline int paged_io_bytes(int type) { return type == PQA_PAGED_F32 ? 4 : 2; }

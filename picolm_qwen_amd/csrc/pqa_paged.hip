@@ -269,13 +269,14 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
         s.wide_wgs = pqa::paged_wide_wgs(p->head_dim, p->cu_count);
         s.wide_rows = pqa::paged_wide_rows(p->type, p->head_dim);
         s.wide_keys = pqa::paged_wide_keys(p->head_dim);
+        s.key_bytes = 4 * p->head_dim;
         s.max_seqs = max_seqs;
         s.max_tokens = max_tokens;
         s.max_seq_pages = (int)(((long long)max_len + p->page_size - 1) / p->page_size);
         b->max_touched = std::min<size_t>((size_t)max_tokens, (size_t)2 * max_seqs + max_tokens / p->page_size);
-        b->max_narrow = (size_t)max_seqs * p->n_kv + s.narrow_wgs;
+        b->max_rest = (size_t)max_seqs * p->n_kv + s.narrow_wgs;
         // blocks of every sequence, and as many parts again
-        b->max_wide = ((size_t)max_tokens * p->group / s.wide_rows + max_seqs) * p->n_kv + s.wide_wgs;
+        b->max_wide = ((size_t)max_tokens * p->group / s.wide_rows + max_seqs) * p->n_kv + 2 * s.wide_wgs;
         const size_t entries = (size_t)max_seqs * s.max_seq_pages;
         // no plan of this capacity leaves more partials: a block of rows is cut into at most max_len / kWideLeast + 1 parts
         const size_t blocks = (size_t)max_tokens * p->group <= pqa::kNarrowRows ? 0 : (size_t)max_tokens * p->group / s.wide_rows + std::min(max_seqs, max_tokens);
@@ -284,10 +285,9 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
             void** p;
             size_t bytes;
         } parts[] = {{(void**)&b->header, pqa::kPagedHeader * 4},
-                     {(void**)&b->seqs, (size_t)max_seqs * sizeof(pqa::PagedSeq)},
-                     {(void**)&b->token_seq, (size_t)max_tokens * 4},
-                     {(void**)&b->narrow_first, ((size_t)s.narrow_wgs + 1) * 4},
-                     {(void**)&b->narrow, b->max_narrow * sizeof(pqa::PagedItem)},
+                     {(void**)&b->runs, (size_t)s.narrow_wgs * sizeof(pqa::PagedRun)},
+                     {(void**)&b->rest, b->max_rest * sizeof(pqa::PagedItem)},
+                     {(void**)&b->tokens, (size_t)max_tokens * sizeof(pqa::PagedToken)},
                      {(void**)&b->wide, b->max_wide * sizeof(pqa::PagedItem)},
                      {(void**)&b->touched, b->max_touched * sizeof(pqa::PagedTouched)},
                      {(void**)&b->pages, entries * 4},
@@ -337,7 +337,7 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         const PagedFault f = pqa::paged_check(s, n_seqs, n_new, len, pages, stride, &plan, &why);
         if (f != PagedFault::none) return fail(p, f == PagedFault::range ? PQA_ERR_RANGE : PQA_ERR_ARG, name + ": " + why);
         pqa::paged_items(s, &plan);
-        if (plan.narrow.size() > b->max_narrow || plan.wide.size() > b->max_wide || plan.touched.size() > b->max_touched)
+        if (plan.runs.size() > (size_t)s.narrow_wgs || plan.rest.size() > b->max_rest || plan.wide.size() > b->max_wide || plan.touched.size() > b->max_touched)
             return fail(p, PQA_ERR_ARG, name + ": plan exceeds the batch");  // cannot happen: the capacities follow from the checks
         OnDevice on(b->device);
         hipStream_t st = (hipStream_t)stream;
@@ -346,16 +346,15 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         if (e == hipSuccess) e = is_captured(st, &captured);
         if (e != hipSuccess) return hip_fail(p, e, name);
         if (captured) return fail(p, PQA_ERR_ARG, name + ": not while the stream is captured (replayed calls follow a later set)");
-        const int header[pqa::kPagedHeader] = {plan.n_tok, (int)plan.touched.size(), (int)plan.wide.size(), 0};
+        const int header[pqa::kPagedHeader] = {plan.n_tok, (int)plan.touched.size(), (int)plan.runs.size(), (int)plan.wide.size()};
         const struct {
             void* dst;
             const void* src;
             size_t bytes;
         } parts[] = {{b->header, header, sizeof header},
-                     {b->seqs, plan.seqs.data(), plan.seqs.size() * sizeof(pqa::PagedSeq)},
-                     {b->token_seq, plan.token_seq.data(), plan.token_seq.size() * 4},
-                     {b->narrow_first, plan.narrow_first.data(), plan.narrow_first.size() * 4},
-                     {b->narrow, plan.narrow.data(), plan.narrow.size() * sizeof(pqa::PagedItem)},
+                     {b->runs, plan.runs.data(), plan.runs.size() * sizeof(pqa::PagedRun)},
+                     {b->rest, plan.rest.data(), plan.rest.size() * sizeof(pqa::PagedItem)},
+                     {b->tokens, plan.tokens.data(), plan.tokens.size() * sizeof(pqa::PagedToken)},
                      {b->wide, plan.wide.data(), plan.wide.size() * sizeof(pqa::PagedItem)},
                      {b->touched, plan.touched.data(), plan.touched.size() * sizeof(pqa::PagedTouched)},
                      {b->pages, plan.pages.data(), plan.pages.size() * 4}};

@@ -18,8 +18,7 @@ struct PagedAppend {
     char* kp;  // the layer's pages
     char* vp;
     const int* header;
-    const int* token_seq;
-    const PagedSeq* seqs;
+    const PagedToken* tokens;
     const int* pages;
     const float* qn;  // [head_dim] or null
     const float* kn;
@@ -50,8 +49,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppend a) 
         const int tok = (int)(u / heads), h = (int)(u - (long long)tok * heads);
         const int kind = h < a.nh ? 0 : h < a.nh + a.n_kv ? 1 : 2;  // q, k, v
         const int head = kind == 0 ? h : kind == 1 ? h - a.nh : h - a.nh - a.n_kv;
-        const PagedSeq sq = a.seqs[a.token_seq[tok]];
-        const int pos = sq.len - sq.n_new + tok - sq.row0;
+        const int table = a.tokens[tok].table, pos = a.tokens[tok].pos;
         const Io* src = kind == 0   ? (const Io*)a.q + (long long)tok * a.ldq
                         : kind == 1 ? (const Io*)a.k + (long long)tok * a.ldk
                                     : (const Io*)a.v + (long long)tok * a.ldv;
@@ -67,7 +65,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppend a) 
                 ss = fmaf(y.x, y.x, fmaf(y.y, y.y, fmaf(y.z, y.z, fmaf(y.w, y.w, ss))));
             }
         }
-        const int page = kind == 0 ? 0 : a.pages[sq.table + (pos >> a.shift)];
+        const int page = kind == 0 ? 0 : a.pages[table + (pos >> a.shift)];
         wave_sync();
         if (kind != 2) {
             const float* nw = kind == 0 ? a.qn : a.kn;
@@ -199,12 +197,12 @@ hipError_t launch_append(const pqa_batch* b, int layer, const PagedAppend& a, bo
     const pqa_paged* p = b->p;
     const long long most = 8LL * p->cu_count;  // workgroups; more work takes further turns
     const long long rows = (long long)b->plan.n_tok * (p->n_heads + 2 * p->n_kv);
-    const unsigned grid = (unsigned)(captured ? most : std::min(most, (rows + 15) / 16));
+    const unsigned grid = (unsigned)(captured ? most : std::min(1LL << 30, (rows + 15) / 16));
     hipLaunchKernelGGL((paged_append_kernel<TYPE, HD>), dim3(grid), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p->bounds) return e;
     const long long units = (long long)b->plan.touched.size() * p->n_kv;
-    const unsigned bgrid = (unsigned)(captured ? most : std::min(most, units));
+    const unsigned bgrid = (unsigned)(captured ? most : std::min(1LL << 30, units));
     hipLaunchKernelGGL((paged_bounds_kernel<TYPE, HD>), dim3(bgrid), dim3(256), 0, s, (const char*)a.kp,
                        p->bounds + (size_t)layer * p->layer_heads * 2 * HD, p->scales + (size_t)layer * p->layer_heads, a.header,
                        (const PagedTouched*)b->touched, p->n_kv, p->page_shift);
@@ -239,8 +237,7 @@ hipError_t launch_paged_append(const pqa_batch* b, int layer, const PagedRows& q
     a.kp = p->k + (size_t)layer * p->layer_bytes;
     a.vp = p->v + (size_t)layer * p->layer_bytes;
     a.header = b->header;
-    a.token_seq = b->token_seq;
-    a.seqs = b->seqs;
+    a.tokens = b->tokens;
     a.pages = b->pages;
     if (p->has_qk_norm[layer]) {
         a.qn = p->qk_norm + (size_t)layer * 2 * hd;

@@ -47,14 +47,13 @@ struct PagedAttn {
     const char* kp;  // the layer's pages
     const char* vp;
     const int* pages;
-    const int* items;  // PagedItem
-    const int* first;
+    const int* items;  // PagedItem: the wide ones, or those behind the runs' first
+    const int* runs;   // PagedRun
     const int* header;
     float* part;
     unsigned* counters;
     const int* chosen;  // attention over chosen pages: [token][kv head][select], else null
-    const int* token_seq;
-    const int* seqs;  // PagedSeq
+    const int* tokens;  // PagedToken
     int select, wgs;
     int g, n_kv, shift;
     int qvec, ovec;  // rows may move as 16-byte vectors
@@ -556,7 +555,7 @@ template <int HD>
 constexpr int narrow_waves() { return HD <= 128 ? 4 : 2; }
 
 // ---- up to 16 rows: waves on different key tiles ----
-template <int TYPE, int HD>
+template <int TYPE, int HD, bool STREAM>
 __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
     typedef Geo<HD> G;
     typedef typename PagedType<TYPE>::Io Io;
@@ -592,16 +591,20 @@ __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void pag
     // the work: a run of the plan's items, or (chosen pages) columns of one token, KV head and 16
     // of its heads, each in as many parts as leave no workgroup idle
     const int n_blk = (a.g + 15) / 16;
-    int it, it_end, it_step, parts = 1, cols = 0;
+    int it, it_end, it_step, rest, parts = 1, cols = 0;
     if (a.chosen) {
         cols = scalar_int(a.header, kHdTokens) * a.n_kv * n_blk;
         parts = chosen_parts(a.wgs, cols, a.select, a.shift);
         it = blockIdx.x;
         it_end = cols * parts;
         it_step = gridDim.x;
+        rest = 0;
     } else {
-        it = scalar_int(a.first, blockIdx.x);
-        it_end = scalar_int(a.first, blockIdx.x + 1);
+        if ((int)blockIdx.x >= scalar_int(a.header, kHdRuns)) return;
+        const int* run = a.runs + (size_t)blockIdx.x * (sizeof(PagedRun) / 4);
+        it = 0;
+        it_end = scalar_int(run, 0);
+        rest = scalar_int(run, 1);
         it_step = 1;
     }
     for (; it < it_end; it += it_step) {
@@ -611,15 +614,13 @@ __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void pag
             const int col = it / parts;
             part = it - col * parts;
             const int blk = col % n_blk, tk = col / n_blk, tok = tk / a.n_kv;
-            const int sq4 = 4 * scalar_int(a.token_seq, tok);
-            const int row0 = scalar_int(a.seqs, sq4), n_new = scalar_int(a.seqs, sq4 + 1), len = scalar_int(a.seqs, sq4 + 2);
-            const int pos = len - n_new + tok - row0;
+            const int pos = scalar_int(a.tokens, 4 * tok + 1);
             const int seen = min(a.select, (pos >> a.shift) + 1);  // pages, the last of them the token's own
             c.kend = ((seen - 1) << a.shift) + (pos & ((1 << a.shift) - 1)) + 1;
             c.row0 = tok;
             c.rows = a.g;
             c.hist = c.kend - 1;
-            c.table = scalar_int(a.seqs, sq4 + 3);
+            c.table = scalar_int(a.tokens, 4 * tok);
             c.kvh = tk - tok * a.n_kv;
             c.r0 = 16 * blk;
             c.list = a.chosen + (size_t)tk * a.select;
@@ -629,7 +630,8 @@ __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void pag
             slot0 = col * parts;
             counter = col;
         } else {
-            const int* p = a.items + (size_t)it * (sizeof(PagedItem) / 4);
+            const int* p = it == 0 ? a.runs + (size_t)blockIdx.x * (sizeof(PagedRun) / 4) + 4
+                                   : a.items + (size_t)(rest + it - 1) * (sizeof(PagedItem) / 4);
             c.row0 = scalar_int(p, 0);
             c.rows = scalar_int(p, 1);
             c.hist = scalar_int(p, 2);
@@ -670,7 +672,8 @@ __global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void pag
                             const int L = 64 * i + lane, r = L / G::CH;
                             off = min(r, last) * G::ROWB + 16 * ((L % G::CH) ^ (o ? G::xv(r) : G::xk(r)));
                         }
-                        lds_dma_b128(src, off, lds_addr(&lds[w][buf][o][b * G::BLKB + 1024 * i]));
+                        if constexpr (STREAM) lds_dma_b128_nt(src, off, lds_addr(&lds[w][buf][o][b * G::BLKB + 1024 * i]));
+                        else lds_dma_b128(src, off, lds_addr(&lds[w][buf][o][b * G::BLKB + 1024 * i]));
                     }
                 }
             }
@@ -757,7 +760,7 @@ constexpr int wide_keys() { return HD > 192 ? 32 : 64; }
 
 // ---- more rows: 4 waves share each key tile, RB blocks of 16 rows each ----
 template <int TYPE, int HD>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_wide_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_wide_kernel(const PagedAttn a) {
     typedef Geo<HD> G;
     typedef typename PagedType<TYPE>::Io Io;
     constexpr int KEYS = wide_keys<HD>(), KB = KEYS / 16, RB = wide_blocks<TYPE, HD>(), ROWS = 64 * RB;
@@ -879,9 +882,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_wide_kernel(cons
 }
 
 template <int TYPE, int HD>
-hipError_t launch_kernels(const PagedAttn& a, PagedAttn wide, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     if (narrow_grid) {
-        hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD>), dim3((unsigned)narrow_grid), dim3(64 * narrow_waves<HD>()), 0, s, a);
+        const dim3 grid((unsigned)narrow_grid), block(64 * narrow_waves<HD>());
+        if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, false>), grid, block, 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -893,20 +898,20 @@ hipError_t launch_kernels(const PagedAttn& a, PagedAttn wide, int narrow_grid, i
 }
 
 template <int TYPE>
-hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (hd) {
-#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, narrow_grid, wide_grid, s);
+#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, stream, narrow_grid, wide_grid, s);
         PQA_PG(64) PQA_PG(96) PQA_PG(128) PQA_PG(160) PQA_PG(192) PQA_PG(256)
 #undef PQA_PG
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (b->p->type) {
-        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
-        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
-        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
+        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
     }
 }
 
@@ -921,13 +926,12 @@ PagedAttn arguments(const pqa_batch* b, int layer, const PagedRows& q, void* out
     a.kp = p->k + (size_t)layer * p->layer_bytes;
     a.vp = p->v + (size_t)layer * p->layer_bytes;
     a.pages = b->pages;
-    a.items = (const int*)b->narrow;
-    a.first = b->narrow_first;
+    a.items = (const int*)b->rest;
+    a.runs = (const int*)b->runs;
     a.header = b->header;
     a.part = b->part_narrow;
     a.counters = b->counters;
-    a.token_seq = b->token_seq;
-    a.seqs = (const int*)b->seqs;
+    a.tokens = (const int*)b->tokens;
     a.wgs = b->shape.narrow_wgs;
     a.g = p->group;
     a.n_kv = p->n_kv;
@@ -943,7 +947,7 @@ PagedAttn arguments(const pqa_batch* b, int layer, const PagedRows& q, void* out
 int paged_wide_rows(int type, int hd) { return type != PQA_PAGED_F32 && hd <= 128 ? 128 : 64; }
 int paged_wide_keys(int hd) { return hd > 192 ? 32 : 64; }
 int paged_narrow_wgs(int hd, int cu_count) { return hd == 64 ? 2 * cu_count : cu_count; }
-int paged_wide_wgs(int hd, int cu_count) { return hd <= 128 ? 2 * cu_count : cu_count; }
+int paged_wide_wgs(int hd, int cu_count) { return hd == 64 ? 3 * cu_count : hd <= 128 ? 2 * cu_count : cu_count; }
 
 hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q, void* out, long long ldo, bool captured,
                                hipStream_t s) {
@@ -954,9 +958,9 @@ hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q
     wide.counters = b->counters + b->shape.narrow_wgs;
     // A captured call may be replayed with what the batch holds then: both kernels, on grids that
     // any content fits
-    const int n = captured ? b->shape.narrow_wgs : b->plan.narrow_active;
+    const int n = captured ? b->shape.narrow_wgs : (int)b->plan.runs.size();
     const int w = captured ? b->shape.wide_wgs : (int)b->plan.wide.size();
-    return launch_any(b, a, wide, n, w, s);
+    return launch_any(b, a, wide, b->plan.stream, n, w, s);
 }
 
 hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q, int select, const int* chosen, void* out,
@@ -966,7 +970,9 @@ hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q
     a.select = select;
     const long long cols = (long long)b->plan.n_tok * b->p->n_kv * ((b->p->group + 15) / 16);
     const long long grid = captured ? b->shape.narrow_wgs : cols * chosen_parts(a.wgs, (int)cols, select, a.shift);
-    return launch_any(b, a, a, (int)std::min<long long>(grid, 1 << 30), 0, s);
+    // chosen pages of single tokens are read once, those of a chunk's tokens by many of them
+    const bool stream = b->plan.n_tok == (int)b->plan.seqs.size() && cols * ((long long)select << a.shift) * 4 * b->p->head_dim > kStreamBytes;
+    return launch_any(b, a, a, stream, (int)std::min<long long>(grid, 1 << 30), 0, s);
 }
 
 }  // namespace pqa

@@ -7,9 +7,13 @@
 // by 16 heads at a time; it is a whole number below 2^22 and the scales are powers of two, so
 // every score is exact and the choice is the same in any order of summation.
 //
-// A workgroup per token and KV head: scores to LDS as integers in the floats' order, the
-// threshold by counting digits from the top, then the list in ascending order (the lower
-// page where scores are equal). Bound by reading the bounds, 2 head_dim + 4 bytes per page and KV head.
+// A workgroup takes a KV head of one token, or of as many tokens of a chunk as fill the 16 columns
+// of a product (they share each page's bounds): scores to LDS as integers in the floats' order, then per token
+// the least chosen key and the list in ascending order (the lower page where scores are equal). Up to
+// kWaveKeys pages a wave keeps a token's keys in registers and finds that key bit by bit,
+// counting by ballots (no barrier); longer lists go through the whole workgroup, by digits.
+// Bound by reading the bounds, 2 head_dim + 4 bytes per page and KV head, and for single tokens
+// by the latency of that.
 #include <algorithm>
 
 #include "pqa_paged_device.h"
@@ -26,31 +30,28 @@ struct PagedChoose {
     const int8_t* bounds;  // the layer's
     const float* scales;
     const int* header;
-    const int* token_seq;
-    const PagedSeq* seqs;
+    const int* tokens;  // PagedToken
     const int* pages;
     int* chosen;
     int g, n_kv, shift, select, first, last, qvec;
+    int group, stride;  // tokens per workgroup; keys per token in LDS
 };
 
-constexpr int kChooseThreads = 256, kChooseWaves = kChooseThreads / 64;
+constexpr int kChooseThreads = 512, kChooseWaves = kChooseThreads / 64;
+constexpr int kWaveKeys = 1024;
+constexpr int kChooseBytes = 40 << 10;  // of LDS for the keys, where more than one token shares a workgroup
 
-// 16 elements of a query row as whole numbers of 2^(e - 6), those of one sign (neg: the
-// negative ones), the others as zero
-template <class Io>
-__device__ __forceinline__ intx4 signed_bytes(const Io* p, bool vec, float up, bool neg) {
+// 16 elements as whole numbers, rounded to nearest even, of one sign within [lo, hi] and the others as
+// zero: past 3 * 2^22 a float's step is one, and its low byte the number in two's complement
+__device__ __forceinline__ intx4 signed_bytes(const float (&x)[16], float up, float lo, float hi) {
     intx4 out;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-        const float4 y = load4(p + 4 * w, vec);
-        const float v[4] = {y.x, y.y, y.z, y.w};
-        int word = 0;
+        unsigned b[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float r = fminf(fmaxf(rintf(v[e] * up), neg ? -127.0f : 0.0f), neg ? 0.0f : 127.0f);
-            word |= ((int)r & 0xFF) << (8 * e);
-        }
-        out[w] = word;
+        for (int e = 0; e < 4; e++) b[e] = __float_as_uint(__builtin_amdgcn_fmed3f(x[4 * w + e] * up, lo, hi) + 12582912.0f);
+        const unsigned ab = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), cd = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+        out[w] = (int)(ab | cd);
     }
     return out;
 }
@@ -61,188 +62,282 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ int popcount(unsigned long long x) { return (int)__popcll(x); }
+
+// A token's keys: its forced pages, [0, first) and [p1, n), above all scores.
+struct Keys {
+    const uint32_t* k;
+    int first, p1, n;
+    __device__ uint32_t operator[](int i) const { return i < first || i >= p1 ? 0xFFFFFFFFu : k[i]; }
+};
+
+// The list of one token by one wave; n <= kWaveKeys.
+__device__ __forceinline__ void choose_by_wave(const Keys& keys, int select, int lane, int* out) {
+    constexpr int R = kWaveKeys / 64;
+    uint32_t k[R];
+    const int regs = (keys.n + 63) / 64;
+#pragma unroll
+    for (int r = 0; r < R; r++) k[r] = r < regs && 64 * r + lane < keys.n ? keys[64 * r + lane] : 0u;
+    auto count = [&](uint32_t least) {
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (r < regs) c += popcount(__ballot(k[r] >= least));
+        return c;
+    };
+    // the bits that all scores share (the forced pages' keys are above them anyway)
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (r < regs && 64 * r + lane >= keys.first && 64 * r + lane < keys.p1) {
+            lo = min(lo, k[r]);
+            hi = max(hi, k[r]);
+        }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
+        hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    // the largest key that at least `select` keys reach
+    const int top = lo == hi ? -1 : 31 - __clz((int)(lo ^ hi));  // the highest bit in which two scores differ
+    uint32_t least = top < 0 ? lo : top == 31 ? 0u : lo >> (top + 1) << (top + 1);
+    int reach = count(least);
+#pragma unroll 1
+    for (int bit = top; bit >= 0 && reach != select; bit--) {
+        const uint32_t cand = least | 1u << bit;
+        const int c = count(cand);
+        if (c >= select) {
+            least = cand;
+            reach = c;
+        }
+    }
+    // above it all, of those that equal it the first `same`
+    int same = reach == select ? keys.n : select - (least == 0xFFFFFFFFu ? 0 : count(least + 1)), put = 0;
+    const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (r >= regs) break;
+        const bool in = 64 * r + lane < keys.n, is = in && k[r] == least;
+        const unsigned long long equal = __ballot(is);
+        const bool take = in && (k[r] > least || (is && popcount(equal & below) < same));
+        const unsigned long long taken = __ballot(take);
+        const int to = put + popcount(taken & below);
+        if (take && to < select) out[to] = 64 * r + lane;
+        put += popcount(taken);
+        same = max(0, same - popcount(equal));
+    }
+}
+
 template <int TYPE, int HD>
-__global__ __launch_bounds__(kChooseThreads) void paged_choose_kernel(const PagedChoose a) {
+__global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choose_kernel(const PagedChoose a) {
     typedef typename PagedType<TYPE>::Io Io;
-    constexpr int ST = HD / 32;  // steps of 64 products
-    constexpr int PB = 2;        // blocks of 16 pages at a time
-    extern __shared__ uint32_t keys[];
+    constexpr int ST = HD / 32;              // steps of 64 products
+    constexpr int PB = HD <= 128 ? 4 : 2;    // blocks of 16 pages at a time
+    extern __shared__ uint32_t lds_keys[];
     __shared__ int hist[256];
     __shared__ uint32_t s_lo[kChooseWaves], s_hi[kChooseWaves];
     __shared__ int s_digit, s_left, s_gt[kChooseWaves], s_eq[kChooseWaves];
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g16 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int cols = scalar_int(a.header, kHdTokens) * a.n_kv;
-    for (int col = blockIdx.x; col < cols; col += gridDim.x) {
-        const int tok = col / a.n_kv, kvh = col - tok * a.n_kv;
-        const PagedSeq sq = a.seqs[scalar_int(a.token_seq, tok)];
-        const int own = __builtin_amdgcn_readfirstlane((sq.len - sq.n_new + tok - sq.row0) >> a.shift);
-        const int table = __builtin_amdgcn_readfirstlane(sq.table);
-        const int n = own + 1;
-        int* out = a.chosen + (size_t)col * a.select;
-        if (n <= a.select) {  // every page
-            for (int i = tid; i < a.select; i += kChooseThreads) out[i] = i < n ? i : -1;
-            continue;
-        }
-        // scores of pages [first, n - last), in blocks of 16 PB; the heads in blocks of 16
-        const int p0 = a.first, p1 = n - a.last;
-        for (int i = tid; i < n; i += kChooseThreads)
-            if (i < p0 || i >= p1) keys[i] = 0xFFFFFFFFu;
-        uint32_t lo = 0xFFFFFFFFu, hi = 0;
-        for (int h0 = 0; h0 < a.g; h0 += 16) {
-            const int h = min(h0 + c16, a.g - 1);  // heads past the last one: that one again
-            const Io* q = (const Io*)a.q + (long long)tok * a.ldq + (long long)(kvh * a.g + h) * HD;
-            float mx = 0.0f;
+    // the tokens whose number is a multiple of the group come first, in one run: most of the others
+    // leave at once, and would leave CUs idle in between
+    const int n_tok = scalar_int(a.header, kHdTokens), heads = (n_tok + a.group - 1) / a.group;
+    for (int u = blockIdx.x; u < heads * a.group * a.n_kv; u += gridDim.x) {
+        const int kvh = u % a.n_kv, v = u / a.n_kv, tok = v % heads * a.group + v / heads;
+        if (tok >= n_tok) continue;
+        const int* token = a.tokens + 4 * (size_t)tok;
+        const int table = scalar_int(token, 0), pos = scalar_int(token, 1);
+        if (scalar_int(token, 2) % a.group) continue;  // another token's workgroup has it
+        const int nt = min(a.group, scalar_int(token, 3));
+        const int top = ((pos + nt - 1) >> a.shift) + 1;  // pages that the last of the tokens sees
+        if (top > a.select) {
+            for (int i = tid; i < nt * a.stride; i += kChooseThreads) lds_keys[i] = 0u;
+            __syncthreads();
+            // scores of pages [p0, p1); 16 columns: heads of the tokens, or 16 heads at a time
+            const int p0 = a.first, p1 = top - a.last;
+            for (int h0 = 0; h0 < a.g; h0 += 16) {
+                const int t = a.g > 16 ? 0 : c16 / a.g, h = a.g > 16 ? h0 + c16 : c16 - t * a.g;
+                const bool column = t < nt && h < a.g;  // the others repeat column 0
+                const Io* q = (const Io*)a.q + (long long)(column ? tok + t : tok) * a.ldq + (long long)(kvh * a.g + (column ? h : 0)) * HD;
+                float x[ST][16], mx = 0.0f;
 #pragma unroll
-            for (int st = 0; st < ST; st++) {
-                const int d = 16 * ((4 * st + g16) % (HD / 16));
+                for (int st = 0; st < ST; st++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 y = load4(q + d + 4 * i, a.qvec);
-                    mx = fmaxf(fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+                    for (int i = 0; i < 4; i++) {
+                        const float4 y = load4(q + 16 * ((4 * st + g16) % (HD / 16)) + 4 * i, a.qvec);
+                        x[st][4 * i] = y.x;
+                        x[st][4 * i + 1] = y.y;
+                        x[st][4 * i + 2] = y.z;
+                        x[st][4 * i + 3] = y.w;
+                    }
+#pragma unroll
+                for (int st = 0; st < ST; st++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, fabsf(x[st][i]));
+                const int e = bound_exponent(max_x32(max_x16(mx)));
+                const float up = power2(6 - e), down = power2(e - 6);
+                intx4 qb[ST];
+#pragma unroll
+                for (int st = 0; st < ST; st++) {
+                    const bool neg = 4 * st + g16 < HD / 16;
+                    qb[st] = signed_bytes(x[st], up, neg ? -127.0f : 0.0f, neg ? 0.0f : 127.0f);
                 }
-            }
-            const int e = bound_exponent(max_x32(max_x16(mx)));
-            const float up = power2(6 - e), down = power2(e - 6);
-            intx4 qb[ST];
-#pragma unroll
-            for (int st = 0; st < ST; st++) {
-                const int chunk = 4 * st + g16, d = 16 * (chunk % (HD / 16));
-                qb[st] = signed_bytes(q + d, a.qvec, up, chunk < HD / 16);
-            }
-            for (int b0 = p0 + 16 * PB * w; b0 < p1; b0 += 16 * PB * kChooseWaves) {
-                intx4 x[PB][ST];
+                uint32_t* mine = lds_keys + (column ? t : 0) * a.stride;
                 int page[PB];
+                auto look = [&](int b0) __attribute__((always_inline)) {
 #pragma unroll
-                for (int b = 0; b < PB; b++) page[b] = a.pages[table + min(b0 + 16 * b + c16, p1 - 1)];
+                    for (int b = 0; b < PB; b++) page[b] = a.pages[table + min(b0 + 16 * b + c16, p1 - 1)];
+                };
+                int b0 = p0 + 16 * PB * w;
+                if (b0 < p1) look(b0);
+                for (; b0 < p1; b0 += 16 * PB * kChooseWaves) {
+                    intx4 y[PB][ST];
+                    float sc[PB];
 #pragma unroll
-                for (int b = 0; b < PB; b++) {
-                    const int8_t* r = a.bounds + ((size_t)page[b] * a.n_kv + kvh) * (2 * HD) + 16 * g16;
+                    for (int b = 0; b < PB; b++) {
+                        const size_t at = (size_t)page[b] * a.n_kv + kvh;
+                        const int8_t* r = a.bounds + at * (2 * HD) + 16 * g16;
 #pragma unroll
-                    for (int st = 0; st < ST; st++) x[b][st] = *(const intx4*)(r + 64 * st);
-                }
-                float sc[PB];
-#pragma unroll
-                for (int b = 0; b < PB; b++) sc[b] = a.scales[(size_t)page[b] * a.n_kv + kvh];  // of page b0 + 16 b + c16
-#pragma unroll
-                for (int b = 0; b < PB; b++) {
-                    intx4 acc = {0, 0, 0, 0};
-#pragma unroll
-                    for (int st = 0; st < ST; st++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[b][st], qb[st], acc, 0, 0, 0);
-                    // pages 4 g16 + j of head c16; the lane with c16 = 4 g16 + j keeps that page's
-                    float mine = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float m = group_max<16>((float)acc[j] * down);
-                        if (c16 == 4 * g16 + j) mine = m;
+                        for (int st = 0; st < ST; st++) y[b][st] = *(const intx4*)(r + 64 * st);
+                        sc[b] = a.scales[at];  // of page b0 + 16 b + c16
                     }
-                    const int i = b0 + 16 * b + c16;
-                    if ((c16 >> 2) == g16 && i < p1) {
-                        const uint32_t before = h0 ? keys[i] : 0u;
-                        const uint32_t key = max(before, min(ordered_bits(mine * sc[b]), 0xFFFFFFFEu));
-                        keys[i] = key;
-                        if (h0 + 16 >= a.g) {
-                            lo = min(lo, key);
-                            hi = max(hi, key);
+                    if (b0 + 16 * PB * kChooseWaves < p1) look(b0 + 16 * PB * kChooseWaves);
+#pragma unroll
+                    for (int b = 0; b < PB; b++) {
+                        intx4 acc = {0, 0, 0, 0};
+#pragma unroll
+                        for (int st = 0; st < ST; st++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[b][st], qb[st], acc, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {  // page 4 g16 + j of column c16
+                            const float s = (float)acc[j] * down * __shfl(sc[b], 4 * g16 + j);
+                            const int i = b0 + 16 * b + 4 * g16 + j;
+                            if (column && i < p1) atomicMax(mine + i, min(ordered_bits(s), 0xFFFFFFFEu));
                         }
                     }
                 }
             }
+            __syncthreads();
         }
-        // the range of the scores, so that the first digit tells them apart
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-            hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-        }
-        if (lane == 0) {
-            s_lo[w] = lo;
-            s_hi[w] = hi;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kChooseWaves; i++) {
-            lo = min(lo, s_lo[i]);
-            hi = max(hi, s_hi[i]);
-        }
-        // the `left`-th largest of keys [p0, p1) by digits of 8 bits of key - lo, from the top:
-        // key - lo has `bits` bits, of which those above `shift` are known to be `prefix`
-        const int bits = hi > lo ? 32 - __clz((int)(hi - lo)) : 0;
-        int left = a.select - (n - (p1 - p0));
-        uint32_t prefix = 0;
-        int shift = bits;
-        if (left > 0)
-            while (shift > 0) {
-                const int width = min(8, shift), next = shift - width;
-                hist[tid] = 0;
-                __syncthreads();
-                for (int i = p0 + tid; i < p1; i += kChooseThreads) {
-                    const uint32_t k = keys[i] - lo;
-                    if (shift >= 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> next) & ((1u << width) - 1)], 1);
-                }
-                __syncthreads();
-                if (w == 0) {  // lane l: digits 4 l .. 4 l + 3; the sum of all larger ones by a scan
-                    int c[4], sum = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) sum += c[j] = hist[4 * lane + j];
-                    int above = sum;  // of this lane's digits and all higher lanes'
-#pragma unroll
-                    for (int d = 1; d < 64; d <<= 1) {
-                        const int y = __shfl_down(above, d);
-                        if (lane + d < 64) above += y;
-                    }
-                    int over = above - sum;  // strictly above this lane's digits
-#pragma unroll
-                    for (int j = 3; j >= 0; j--) {
-                        if (over < left && left <= over + c[j]) {
-                            s_digit = 4 * lane + j;
-                            s_left = left - over;
-                        }
-                        over += c[j];
-                    }
-                }
-                __syncthreads();
-                prefix = prefix << width | (uint32_t)s_digit;
-                left = s_left;
-                shift = next;
+        // a list per token: short ones a wave each
+        for (int t = 0; t < nt; t++) {
+            const int n = ((pos + t) >> a.shift) + 1;
+            if (n > a.select && n > kWaveKeys) continue;
+            if (t % kChooseWaves != w) continue;
+            int* out = a.chosen + ((size_t)(tok + t) * a.n_kv + kvh) * a.select;
+            if (n <= a.select) {  // every page
+                for (int i = lane; i < a.select; i += 64) out[i] = i < n ? i : -1;
+            } else {
+                choose_by_wave(Keys{lds_keys + t * a.stride, a.first, n - a.last, n}, a.select, lane, out);
             }
-        // keys above lo + prefix are chosen, and the first `left` that equal it; each wave lists a
-        // run of the pages behind what the waves before it found
-        const uint32_t at = left > 0 ? lo + prefix : 0xFFFFFFFFu;  // left == 0: the forced pages alone
-        const bool none = left <= 0;
-        const int run = (n + kChooseWaves * 64 - 1) / (kChooseWaves * 64) * 64, r0 = w * run, r1 = min(n, r0 + run);
-        int gt = 0, eq = 0;
-        for (int i = r0 + lane; i < r1; i += 64) {
-            const uint32_t k = keys[i];
-            gt += none ? k == 0xFFFFFFFFu : k > at;
-            eq += !none && k == at;
         }
-        for (int d = 32; d; d >>= 1) {
-            gt += __shfl_xor(gt, d);
-            eq += __shfl_xor(eq, d);
-        }
-        if (lane == 0) {
-            s_gt[w] = gt;
-            s_eq[w] = eq;
-        }
-        __syncthreads();
-        int put = 0, same = 0;  // listed, and equal ones met, before this wave's run
-        for (int i = 0; i < w; i++) {
-            put += s_gt[i] + min(s_eq[i], max(0, left - same));
-            same += s_eq[i];
-        }
-        const unsigned long long below = (1ull << lane) - 1;
-        for (int i0 = r0; i0 < r1; i0 += 64) {
-            const int i = i0 + lane;
-            const uint32_t k = i < r1 ? keys[i] : 0u;
-            const bool is = i < r1 && !none && k == at;
-            const unsigned long long equal = __ballot(is);
-            const bool take = i < r1 && ((none ? k == 0xFFFFFFFFu : k > at) || (is && same + __popcll(equal & below) < left));
-            const unsigned long long taken = __ballot(take);
-            const int to = put + __popcll(taken & below);
-            if (take && to < a.select) out[to] = i;
-            put += __popcll(taken);
-            same += __popcll(equal);
+        for (int t = 0; t < nt; t++) {
+            const int n = ((pos + t) >> a.shift) + 1;
+            if (n <= a.select || n <= kWaveKeys) continue;
+            int* out = a.chosen + ((size_t)(tok + t) * a.n_kv + kvh) * a.select;
+            const Keys keys = {lds_keys + t * a.stride, a.first, n - a.last, n};
+            const int p0 = a.first, p1 = n - a.last;
+            // the range of the scores, so that the first digit tells them apart
+            uint32_t lo = 0xFFFFFFFFu, hi = 0;
+            for (int i = p0 + tid; i < p1; i += kChooseThreads) {
+                lo = min(lo, keys.k[i]);
+                hi = max(hi, keys.k[i]);
+            }
+#pragma unroll
+            for (int d = 32; d; d >>= 1) {
+                lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
+                hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
+            }
+            if (lane == 0) {
+                s_lo[w] = lo;
+                s_hi[w] = hi;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kChooseWaves; i++) {
+                lo = min(lo, s_lo[i]);
+                hi = max(hi, s_hi[i]);
+            }
+            // the `left`-th largest of keys [p0, p1) by digits of 8 bits of key - lo, from the top:
+            // key - lo has `bits` bits, of which those above `shift` are known to be `prefix`
+            const int bits = hi > lo ? 32 - __clz((int)(hi - lo)) : 0;
+            int left = a.select - (n - (p1 - p0));
+            uint32_t prefix = 0;
+            int shift = bits;
+            if (left > 0)
+                while (shift > 0) {
+                    const int width = min(8, shift), next = shift - width;
+                    if (tid < 256) hist[tid] = 0;
+                    __syncthreads();
+                    for (int i = p0 + tid; i < p1; i += kChooseThreads) {
+                        const uint32_t k = keys.k[i] - lo;
+                        if (shift >= 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> next) & ((1u << width) - 1)], 1);
+                    }
+                    __syncthreads();
+                    if (w == 0) {  // lane l: digits 4 l .. 4 l + 3; the sum of all larger ones by a scan
+                        int c[4], sum = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sum += c[j] = hist[4 * lane + j];
+                        int above = sum;  // of this lane's digits and all higher lanes'
+#pragma unroll
+                        for (int d = 1; d < 64; d <<= 1) {
+                            const int y = __shfl_down(above, d);
+                            if (lane + d < 64) above += y;
+                        }
+                        int over = above - sum;  // strictly above this lane's digits
+#pragma unroll
+                        for (int j = 3; j >= 0; j--) {
+                            if (over < left && left <= over + c[j]) {
+                                s_digit = 4 * lane + j;
+                                s_left = left - over;
+                            }
+                            over += c[j];
+                        }
+                    }
+                    __syncthreads();
+                    prefix = prefix << width | (uint32_t)s_digit;
+                    left = s_left;
+                    shift = next;
+                }
+            // keys above lo + prefix are chosen, and the first `left` that equal it (left == 0: the
+            // forced pages alone); each wave lists a run of the pages behind what the waves before it found
+            const uint32_t at = left > 0 ? lo + prefix : 0xFFFFFFFEu;
+            const int run = (n + kChooseWaves * 64 - 1) / (kChooseWaves * 64) * 64, r0 = w * run, r1 = min(n, r0 + run);
+            int gt = 0, eq = 0;
+            for (int i = r0 + lane; i < r1; i += 64) {
+                const uint32_t k = keys[i];
+                gt += k > at;
+                eq += k == at;
+            }
+            for (int d = 32; d; d >>= 1) {
+                gt += __shfl_xor(gt, d);
+                eq += __shfl_xor(eq, d);
+            }
+            if (lane == 0) {
+                s_gt[w] = gt;
+                s_eq[w] = eq;
+            }
+            __syncthreads();
+            int put = 0, same = 0;  // listed, and equal ones met, before this wave's run
+            for (int i = 0; i < w; i++) {
+                put += s_gt[i] + min(s_eq[i], max(0, left - same));
+                same += s_eq[i];
+            }
+            const unsigned long long below = (1ull << lane) - 1;
+            for (int i0 = r0; i0 < r1; i0 += 64) {
+                const int i = i0 + lane;
+                const uint32_t k = i < r1 ? keys[i] : 0u;
+                const bool is = i < r1 && k == at;
+                const unsigned long long equal = __ballot(is);
+                const bool take = i < r1 && (k > at || (is && same + popcount(equal & below) < left));
+                const unsigned long long taken = __ballot(take);
+                const int to = put + popcount(taken & below);
+                if (take && to < a.select) out[to] = i;
+                put += popcount(taken);
+                same += popcount(equal);
+            }
+            __syncthreads();
         }
         __syncthreads();  // LDS is free again
     }
@@ -252,7 +347,7 @@ template <int TYPE, int HD>
 hipError_t launch_choose(const PagedChoose& a, unsigned grid, size_t lds, hipStream_t s) {
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void*)paged_choose_kernel<TYPE, HD>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kPagedMaxChoice * 4);
+                                                 (kPagedMaxChoice + 1) * 4);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL((paged_choose_kernel<TYPE, HD>), dim3(grid), dim3(kChooseThreads), lds, s, a);
@@ -281,8 +376,7 @@ hipError_t launch_paged_choose(const pqa_batch* b, int layer, const PagedRows& q
     a.bounds = p->bounds + (size_t)layer * p->layer_heads * 2 * p->head_dim;
     a.scales = p->scales + (size_t)layer * p->layer_heads;
     a.header = b->header;
-    a.token_seq = b->token_seq;
-    a.seqs = b->seqs;
+    a.tokens = (const int*)b->tokens;
     a.pages = b->pages;
     a.chosen = chosen;
     a.g = p->group;
@@ -298,9 +392,11 @@ hipError_t launch_paged_choose(const pqa_batch* b, int layer, const PagedRows& q
         for (const PagedSeq& sq : b->plan.seqs)
             if (sq.n_new) longest = std::max(longest, (sq.len + p->page_size - 1) / p->page_size);
     if (longest > kPagedMaxChoice) return hipErrorInvalidValue;
-    const size_t lds = (size_t)longest * 4;
+    a.stride = longest | 1;  // odd: the tokens' keys of one page lie in different banks
+    a.group = std::max(1, std::min(a.g > 16 ? 1 : 16 / a.g, kChooseBytes / (4 * a.stride)));
+    const size_t lds = (size_t)a.group * a.stride * 4;
     const long long most = 16LL * p->cu_count;
-    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(most, (long long)b->plan.n_tok * p->n_kv));
+    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(1 << 30, ((long long)b->plan.n_tok + a.group) * p->n_kv));
     switch (p->type) {
         case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(p->head_dim, a, grid, lds, s);
         case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(p->head_dim, a, grid, lds, s);

@@ -35,6 +35,15 @@ struct PagedSeq {
     int32_t row0, n_new, len, table;
 };
 
+struct PagedToken {  // a token row: its sequence's page list, its position, its number among the sequence's new ones, and
+    int32_t table, pos, nth, left;  // how many of these there are from it on
+};
+
+struct PagedRun {  // a narrow workgroup's items: the first, and count - 1 more from `rest` on
+    int32_t count, rest, unused[2];
+    PagedItem first;
+};
+
 struct PagedTouched {  // a page that receives rows: its id and the rows in use afterwards
     int32_t page, used;
 };
@@ -44,18 +53,19 @@ struct PagedShape {
     int n_pages, page_size, group, n_kv, max_pos;  // max_pos: positions that the rotation's tables hold; 0: no rotation
     int narrow_wgs;                                // workgroups of the narrow kernel that run at once
     int wide_wgs, wide_rows, wide_keys;            // the same for the wide one, and its tile
+    int key_bytes;                                 // K and V of one position and KV head
     int max_seqs, max_tokens, max_seq_pages;       // what the batch holds; pages of one sequence
 };
 
 struct PagedPlan {
     int n_tok = 0;
     std::vector<PagedSeq> seqs;
-    std::vector<int32_t> token_seq;  // the sequence of each token row
+    std::vector<PagedToken> tokens;
     std::vector<int32_t> pages;
     std::vector<PagedTouched> touched;
-    std::vector<int32_t> narrow_first;  // items of workgroup w: [narrow_first[w], narrow_first[w + 1])
-    std::vector<PagedItem> narrow, wide;
-    int narrow_active = 0;  // workgroups that have an item
+    std::vector<PagedRun> runs;  // of the narrow workgroups that have work
+    std::vector<PagedItem> rest, wide;
+    bool stream = false;  // the narrow items' K and V pass through the caches once
 };
 
 enum class PagedFault { none, argument, range };
@@ -74,7 +84,7 @@ inline PagedFault paged_check(const PagedShape& s, int n_seqs, const int* n_new,
         return f;
     };
     plan->seqs.clear();
-    plan->token_seq.clear();
+    plan->tokens.clear();
     plan->pages.clear();
     plan->touched.clear();
     if (n_seqs < 0 || n_seqs > s.max_seqs) {
@@ -110,7 +120,7 @@ inline PagedFault paged_check(const PagedShape& s, int n_seqs, const int* n_new,
     }
     plan->n_tok = (int)tokens;
     plan->seqs.reserve(n_seqs);
-    plan->token_seq.reserve((size_t)tokens);
+    plan->tokens.reserve((size_t)tokens);
     plan->pages.reserve((size_t)entries);
     // a page that receives rows belongs to one sequence alone: 1 listed, 2 listed and written
     std::vector<char> mark((size_t)s.n_pages, 0);
@@ -143,7 +153,7 @@ inline PagedFault paged_check(const PagedShape& s, int n_seqs, const int* n_new,
     for (int i = 0; i < n_seqs; i++) {
         const int used = (int)(((long long)len[i] + s.page_size - 1) / s.page_size);
         plan->seqs.push_back({row, n_new[i], len[i], (int)plan->pages.size()});
-        plan->token_seq.insert(plan->token_seq.end(), (size_t)n_new[i], i);
+        for (int j = 0; j < n_new[i]; j++) plan->tokens.push_back({(int)plan->pages.size(), len[i] - n_new[i] + j, j, n_new[i] - j});
         plan->pages.insert(plan->pages.end(), pages + (size_t)i * stride, pages + (size_t)i * stride + used);
         if (n_new[i])
             for (int j = (len[i] - n_new[i]) / s.page_size; j < used; j++)
@@ -153,31 +163,62 @@ inline PagedFault paged_check(const PagedShape& s, int n_seqs, const int* n_new,
     return PagedFault::none;
 }
 
+// Which kernel takes a sequence of few rows. Beside chunks the wide one does, as long as its keys are
+// few: one launch, and the chunks' workgroups fill the gaps (3 chunks of 150 to 500 tokens beside 9
+// single ones behind 10 to 4000, 32 / 4 heads of 64: 34.4 us in two launches, 21.2 in one). From
+// kWideBytes on the narrow one's rate is worth its launch (48 tokens behind 345k positions of 32 / 8 heads
+// of 128: 314 us wide, 204 narrow, a difference of 1 us per 13 MB).
+constexpr long long kWideBytes = 96LL << 20;
+// Without chunks, K and V of this many bytes go past the L2s (32 MB in all), which then keep what the
+// call reads again: 131072 keys of 8 heads of 128 (537 MB) 100 -> 89 us, the 48 tokens above 204 -> 182. Below, a
+// caller that comes back to the same layer soon finds them there: 700 keys of 2 heads of 64 8.4
+// us, past the caches 9.3.
+constexpr long long kStreamBytes = 48LL << 20;
+
 // The narrow items: the key tiles of all (sequence, KV head) columns laid end to end and cut
 // into a run per workgroup. A column costs its tiles and kNarrowOverhead more (q, the joining
 // of the waves, the write), a run has at least kNarrowLeast tiles (one per wave), and a cut
-// leaves at least that much on both sides.
+// leaves at least that much on both sides. Where no column is longer than kNarrowWhole tiles none is
+// cut below its length: joining parts costs what those tiles do.
 constexpr int kNarrowOverhead = 8;
 constexpr int kNarrowLeast = 4;
+constexpr int kNarrowWhole = 24;
 
-// The wide items: blocks of wide_rows rows, cut along the keys only where the blocks leave
-// workgroups idle, into parts of at least kWideLeast keys; the longest first.
+// The wide items: blocks of wide_rows rows, longest first, cut along the keys into parts of about an
+// even share of all blocks' tiles and at least kWideLeast keys.
 constexpr int kWideLeast = 512;
 
 inline void paged_items(const PagedShape& s, PagedPlan* plan) {
-    plan->narrow.clear();
+    plan->runs.clear();
+    plan->rest.clear();
     plan->wide.clear();
-    plan->narrow_first.assign((size_t)s.narrow_wgs + 1, 0);
-    plan->narrow_active = 0;
-    long long cost = 0;
-    for (const PagedSeq& q : plan->seqs)
-        if (q.n_new && (long long)q.n_new * s.group <= kNarrowRows)
-            cost += (long long)s.n_kv * ((q.len + kNarrowKeys - 1) / kNarrowKeys + kNarrowOverhead);
+    std::vector<PagedItem> items;
+    std::vector<int> first;  // of each workgroup
+    long long cost = 0, bytes = 0;
+    int longest = 0;
+    bool chunks = false;
+    for (const PagedSeq& q : plan->seqs) {
+        if (!q.n_new) continue;
+        if ((long long)q.n_new * s.group > kNarrowRows) {
+            chunks = true;
+            continue;
+        }
+        const int tiles = (q.len + kNarrowKeys - 1) / kNarrowKeys;
+        longest = std::max(longest, tiles);
+        cost += (long long)s.n_kv * (tiles + kNarrowOverhead);
+        bytes += (long long)s.n_kv * q.len * s.key_bytes;
+    }
+    const bool narrow = cost && (!chunks || bytes > kWideBytes);
+    plan->stream = narrow && bytes > kStreamBytes;
+    // the rows that the narrow kernel takes
+    auto is_narrow = [&](const PagedSeq& q) { return narrow && (long long)q.n_new * s.group <= kNarrowRows; };
     int counter = 0;
-    if (cost) {
+    if (narrow) {
+        first.push_back(0);
         // The least share that the workgroups can take all of: cuts cost more than the columns alone,
         // so an even share of these is tried first and then grown.
         long long share = std::max<long long>((cost + s.narrow_wgs - 1) / s.narrow_wgs, kNarrowLeast + kNarrowOverhead);
+        if (longest <= kNarrowWhole) share = std::max<long long>(share, longest + kNarrowOverhead);
         // what a workgroup takes of a column's `left` tiles with `room` to go; 0: nothing
         auto piece = [](long long room, int left) {
             const long long take = room - kNarrowOverhead;
@@ -187,7 +228,7 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
             int need = 1;
             long long room = share;
             for (const PagedSeq& q : plan->seqs) {
-                if (!q.n_new || (long long)q.n_new * s.group > kNarrowRows) continue;
+                if (!q.n_new || !is_narrow(q)) continue;
                 const int tiles = (q.len + kNarrowKeys - 1) / kNarrowKeys;
                 for (int kvh = 0; kvh < s.n_kv && need <= s.narrow_wgs; kvh++)
                     for (int t = 0; t < tiles;) {
@@ -202,28 +243,28 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
             }
             if (need <= s.narrow_wgs) break;
         }
-        int w = 0, slot = 0;
+        int slot = 0;
         long long room = share;
         for (const PagedSeq& q : plan->seqs) {
-            if (!q.n_new || (long long)q.n_new * s.group > kNarrowRows) continue;
+            if (!q.n_new || !is_narrow(q)) continue;
             const int tiles = (q.len + kNarrowKeys - 1) / kNarrowKeys;
             for (int kvh = 0; kvh < s.n_kv; kvh++) {
-                const size_t begin = plan->narrow.size();
+                const size_t begin = items.size();
                 for (int t = 0; t < tiles;) {
                     const int take = piece(room, tiles - t);
                     if (!take) {  // no room for a piece: the next workgroup
-                        plan->narrow_first[++w] = (int)plan->narrow.size();
+                        first.push_back((int)items.size());
                         room = share;
                         continue;
                     }
-                    plan->narrow.push_back({q.row0, q.n_new * s.group, q.len - q.n_new, q.table, kvh, 0, t, t + take, 0, 0, 1, 0});
+                    items.push_back({q.row0, q.n_new * s.group, q.len - q.n_new, q.table, kvh, 0, t, t + take, 0, 0, 1, 0});
                     t += take;
                     room -= take + kNarrowOverhead;
                 }
-                const int parts = (int)(plan->narrow.size() - begin);
+                const int parts = (int)(items.size() - begin);
                 if (parts > 1) {
                     for (int p = 0; p < parts; p++) {
-                        PagedItem& it = plan->narrow[begin + p];
+                        PagedItem& it = items[begin + p];
                         it.slot0 = slot;
                         it.part = p;
                         it.parts = parts;
@@ -234,8 +275,11 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
                 }
             }
         }
-        plan->narrow_active = w + 1;
-        for (int i = w + 1; i <= s.narrow_wgs; i++) plan->narrow_first[i] = (int)plan->narrow.size();
+        first.push_back((int)items.size());
+        for (size_t w = 0; w + 1 < first.size(); w++) {
+            plan->runs.push_back({first[w + 1] - first[w], (int)plan->rest.size(), {0, 0}, items[first[w]]});
+            plan->rest.insert(plan->rest.end(), items.begin() + first[w] + 1, items.begin() + first[w + 1]);
+        }
     }
     // wide
     struct Block {
@@ -246,7 +290,7 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
     for (size_t i = 0; i < plan->seqs.size(); i++) {
         const PagedSeq& q = plan->seqs[i];
         const long long rows = (long long)q.n_new * s.group;
-        if (rows <= kNarrowRows) continue;
+        if (!rows || is_narrow(q)) continue;
         for (int r0 = 0; r0 < rows; r0 += s.wide_rows) {
             const int last = (int)std::min<long long>(rows, (long long)r0 + s.wide_rows) - 1;
             const int keys = q.len - q.n_new + last / s.group + 1;
@@ -257,15 +301,14 @@ inline void paged_items(const PagedShape& s, PagedPlan* plan) {
     }
     if (blocks.empty()) return;
     std::stable_sort(blocks.begin(), blocks.end(), [](const Block& a, const Block& b) { return a.tiles > b.tiles; });
-    const long long wgs = (long long)blocks.size() * s.n_kv;
-    long long target = total;  // tiles of a part: no cut
-    if (wgs < s.wide_wgs) target = std::max<long long>((total * s.n_kv + s.wide_wgs - 1) / s.wide_wgs, kWideLeast / s.wide_keys);
+    // tiles of a part: an even share of all
+    const long long target = std::max<long long>((total * s.n_kv + s.wide_wgs - 1) / s.wide_wgs, kWideLeast / s.wide_keys);
     counter = 0;
     int slot = 0;
     for (const Block& b : blocks) {
         const PagedSeq& q = plan->seqs[b.seq];
-        // rounded down, the parts of all blocks are at most total / target <= wide_wgs, and one for each block
-        const int parts = (int)std::max<long long>(1, b.tiles / target);
+        // to the nearest: the cut blocks' parts are at most 4/3 of wide_wgs in all
+        const int parts = (int)std::max<long long>(1, (b.tiles + target / 2) / target);
         for (int p = 0; p < parts; p++)
             for (int kvh = 0; kvh < s.n_kv; kvh++) {
                 PagedItem it = {q.row0, q.n_new * s.group, q.len - q.n_new, q.table, kvh, b.r0,

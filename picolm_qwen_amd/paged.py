@@ -147,6 +147,9 @@ class PagedAttention:
         self._check(rc)
         self._h = h
         self._calls = lib()
+        # one call costs the host some 3 us; what the wrapper looks up each time is kept short
+        self._empty_like, self._zeros_like = torch.empty_like, torch.zeros_like
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if rope_cos is not None or rope_sin is not None or rope_base is not None:
             self.set_rope(rope_style, rot_dim, rope_base, max_pos, rope_cos, rope_sin)
 
@@ -192,6 +195,8 @@ class PagedAttention:
             raise PQAError(rc, msg.decode() if msg else "")
 
     def _stream(self) -> int:
+        if self._raw_stream is not None:
+            return self._raw_stream(self._index)
         import torch
 
         return torch.cuda.current_stream(self._device).cuda_stream
@@ -242,28 +247,33 @@ class PagedAttention:
     def _rows(self, t, dim: int, n: int, what: str):
         """(address, row distance) of token rows the library reads or writes n of; anything that would make a kernel leave the
         tensor raises."""
+        shape, stride = t.shape, t.stride()
+        if (len(shape) != 2 or shape[1] != dim or shape[0] < n or stride[1] != 1 or stride[0] < dim
+                or t.dtype is not self.io_type or t.get_device() != self._index):
+            return self._unusual_rows(t, dim, n, what)
+        return t.data_ptr(), stride[0]
+
+    def _unusual_rows(self, t, dim: int, n: int, what: str):
         if t.dim() != 2 or t.shape[1] != dim or t.shape[0] < n:
             raise ValueError(f"{what}: expected at least {n} rows of {dim}, got {tuple(t.shape)}")
         if t.dtype != self.io_type:
             raise ValueError(f"{what}: expected {self.io_type}, got {t.dtype}")
         if t.get_device() != self._index:
             raise ValueError(f"{what} must be on the cache's GPU")
-        s0, s1 = t.stride()
-        if s1 != 1 or (s0 < dim and t.shape[0] > 1):
+        if t.stride(1) != 1 or t.shape[0] > 1:
             raise ValueError(f"{what}: elements of a row must lie side by side, rows apart")
-        return t.data_ptr(), max(s0, dim)
+        return t.data_ptr(), dim  # one row, whose distance to the next means nothing
 
-    def _out(self, out, q, batch):
-        if out is None:
-            # rows behind the batch's last token are not written
-            return q.new_empty(q.shape) if q.shape[0] == batch.n_tokens else q.new_zeros(q.shape)
-        return out
+    def _out(self, q, batch):
+        # rows behind the batch's last token are not written
+        return self._empty_like(q) if q.shape[0] == batch.n_tokens else self._zeros_like(q)
 
     def append(self, layer: int, batch: PagedBatch, q, k, v, q_out=None):
         """K and V of the batch's new tokens into their pages; returns q normed and rotated (q_out may be q)."""
         n = batch.n_tokens
         a = self._rows(q, self.q_dim, n, "q")
-        q_out = self._out(q_out, q, batch)
+        if q_out is None:
+            q_out = self._out(q, batch)
         rc = self._calls.pqa_paged_append(self.handle, batch.handle, layer, *a, *self._rows(k, self.kv_dim, n, "k"),
                                           *self._rows(v, self.kv_dim, n, "v"), *self._rows(q_out, self.q_dim, n, "q_out"),
                                           self._stream())
@@ -275,7 +285,8 @@ class PagedAttention:
         """Causal attention of the new tokens over their sequences' pages, q as append returns it (out may be q)."""
         n = batch.n_tokens
         a = self._rows(q, self.q_dim, n, "q")
-        out = self._out(out, q, batch)
+        if out is None:
+            out = self._out(q, batch)
         rc = self._calls.pqa_paged_attend(self.handle, batch.handle, layer, *a, *self._rows(out, self.q_dim, n, "out"), self._stream())
         if rc:
             self._check(rc)
@@ -285,7 +296,8 @@ class PagedAttention:
         """append, then attend."""
         n = batch.n_tokens
         a = self._rows(q, self.q_dim, n, "q")
-        out = self._out(out, q, batch)
+        if out is None:
+            out = self._out(q, batch)
         rc = self._calls.pqa_paged_forward(self.handle, batch.handle, layer, *a, *self._rows(k, self.kv_dim, n, "k"),
                                            *self._rows(v, self.kv_dim, n, "v"), *self._rows(out, self.q_dim, n, "out"), self._stream())
         if rc:
@@ -298,7 +310,8 @@ class PagedAttention:
 
         n = batch.n_tokens
         a = self._rows(q, self.q_dim, n, "q")
-        out = self._out(out, q, batch)
+        if out is None:
+            out = self._out(q, batch)
         if chosen is None:
             if select < 1:
                 raise ValueError("select must be positive")

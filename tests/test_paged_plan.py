@@ -34,6 +34,7 @@ static PagedShape shape(int page, int group, int n_kv, int wgs, int rows, int ke
     s.max_seqs = 96;
     s.max_tokens = 8192;
     s.max_seq_pages = 9000;
+    s.key_bytes = 512;
     return s;
 }
 
@@ -54,7 +55,7 @@ static int check(int trial, const PagedShape& s, const PagedPlan& p, const std::
     size_t want = 0, n_blocks = 0;
     for (const PagedSeq& q : p.seqs) {
         const long long r = (long long)q.n_new * s.group;
-        if (!q.n_new || (r > kNarrowRows) != wide) continue;
+        if (!q.n_new || (r > kNarrowRows || p.runs.empty()) != wide) continue;
         for (int kvh = 0; kvh < s.n_kv; kvh++)
             for (int r0 = 0; r0 < r; r0 += rows) {
                 n_blocks++;
@@ -85,7 +86,7 @@ static int check(int trial, const PagedShape& s, const PagedPlan& p, const std::
             }
     }
     CHECK(want == items.size());
-    const size_t most = wide ? ((size_t)s.max_tokens * s.group / s.wide_rows + s.max_seqs) * s.n_kv + s.wide_wgs
+    const size_t most = wide ? ((size_t)s.max_tokens * s.group / s.wide_rows + s.max_seqs) * s.n_kv + 2 * s.wide_wgs
                              : (size_t)s.max_seqs * s.n_kv + s.narrow_wgs;
     CHECK(items.size() <= most);
     return 0;
@@ -121,26 +122,33 @@ int main() {
         const PagedFault f = paged_check(s, n, n_new.data(), len.data(), pages.data(), stride, &p, &why);
         if (f != PagedFault::none) std::printf("%s\n", why.c_str());
         CHECK(f == PagedFault::none);
-        CHECK((int)p.token_seq.size() == p.n_tok && p.n_tok == s.max_tokens - left);
+        CHECK((int)p.tokens.size() == p.n_tok && p.n_tok == s.max_tokens - left);
+        for (const PagedSeq& q : p.seqs)
+            for (int i = 0; i < q.n_new; i++) {
+                const PagedToken& t = p.tokens[q.row0 + i];
+                CHECK(t.table == q.table && t.pos == q.len - q.n_new + i && t.nth == i && t.left == q.n_new - i);
+            }
         CHECK(p.touched.size() <= std::min((size_t)s.max_tokens, (size_t)2 * s.max_seqs + s.max_tokens / page));
         for (const PagedTouched& t : p.touched) CHECK(t.used >= 1 && t.used <= page);
         paged_items(s, &p);
-        CHECK((int)p.narrow_first.size() == s.narrow_wgs + 1 && p.narrow_first[0] == 0);
-        for (int w = 0; w < s.narrow_wgs; w++) CHECK(p.narrow_first[w] <= p.narrow_first[w + 1]);
-        CHECK(p.narrow_first[s.narrow_wgs] == (int)p.narrow.size());
-        for (int w = p.narrow_active; w < s.narrow_wgs; w++) CHECK(p.narrow_first[w] == p.narrow_first[w + 1]);
-        {  // no workgroup has much more than its share of the tiles
-            long long tiles = 0, most = 0;
-            for (int w = 0; w < p.narrow_active; w++) {
-                long long mine = 0;
-                for (int i = p.narrow_first[w]; i < p.narrow_first[w + 1]; i++)
-                    mine += p.narrow[i].t1 - p.narrow[i].t0 + kNarrowOverhead;
-                tiles += mine;
-                most = std::max(most, mine);
+        CHECK((int)p.runs.size() <= s.narrow_wgs);
+        std::vector<PagedItem> items;
+        long long tiles = 0, most = 0;
+        for (const PagedRun& r : p.runs) {
+            CHECK(r.count >= 1 && r.rest >= 0 && (size_t)(r.rest + r.count - 1) <= p.rest.size());
+            long long mine = 0;
+            for (int i = 0; i < r.count; i++) {
+                const PagedItem& it = i ? p.rest[r.rest + i - 1] : r.first;
+                items.push_back(it);
+                mine += it.t1 - it.t0 + kNarrowOverhead;
             }
-            CHECK(most <= tiles / s.narrow_wgs * 1.1 + 2 * (kNarrowOverhead + kNarrowLeast));
+            tiles += mine;
+            most = std::max(most, mine);
         }
-        if (check(trial, s, p, p.narrow, false) || check(trial, s, p, p.wide, true)) return 1;
+        CHECK(items.size() == p.rest.size() + p.runs.size());
+        // no workgroup has much more than its share of the tiles (or one whole short column)
+        CHECK(most <= tiles / s.narrow_wgs * 1.1 + 2 * (kNarrowOverhead + kNarrowLeast) + kNarrowWhole);
+        if (check(trial, s, p, items, false) || check(trial, s, p, p.wide, true)) return 1;
         // what pqa_batch_create holds for the wide kernel's partials of this very batch
         size_t blocks = 0, cut = 0;
         int longest = 0, rows = 0;
