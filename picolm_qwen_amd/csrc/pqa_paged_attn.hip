@@ -55,6 +55,7 @@ struct PagedAttn {
     const int* chosen;  // attention over chosen pages: [token][kv head][select], else null
     const int* tokens;  // PagedToken
     int select, wgs;
+    int crowd;  // chosen pages of many columns: workgroups of two waves, so that two share a CU
     int g, n_kv, shift;
     int qvec, ovec;  // rows may move as 16-byte vectors
     float qscale;
@@ -471,21 +472,6 @@ __device__ __forceinline__ float2 part_load2(const float* p) {
     return float2{__uint_as_float((unsigned)u), __uint_as_float((unsigned)(u >> 32))};
 }
 
-// Called by the whole workgroup after its part's stores; true in the workgroup that finishes
-// last, which then sees all parts. Its counter is zero again for the next call.
-__device__ __forceinline__ bool last_of(unsigned* counter, int parts, int* flag) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have reached memory
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = n == (unsigned)parts - 1;
-        if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    asm volatile("" ::: "memory");  // the loads of the parts stay behind the counter
-    return *flag != 0;
-}
-
 // Joins the parts of `rows` rows in the order of the parts. lds: BYTES of the workgroup's LDS; the
 // rows go in groups whose maxima and sums fit it. Where a group has fewer elements
 // than the workgroup threads, several threads share an element's parts.
@@ -547,6 +533,7 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const Column& c, 
 __host__ __device__ inline int chosen_parts(int wgs, int cols, int select, int shift) {
     if (cols <= 0) return 1;
     const long long keys = (long long)select << shift, piece = kNarrowKeys * kNarrowLeast;
+    if (keys <= kNarrowKeys * kNarrowWhole) return 1;
     const long long most = (keys + piece - 1) / piece, room = wgs / cols;
     return (int)(room < 1 ? 1 : room < most ? room : most);
 }
@@ -555,11 +542,11 @@ template <int HD>
 constexpr int narrow_waves() { return HD <= 128 ? 4 : 2; }
 
 // ---- up to 16 rows: waves on different key tiles ----
-template <int TYPE, int HD, bool STREAM>
-__global__ __launch_bounds__(64 * narrow_waves<HD>(), HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
+template <int TYPE, int HD, int KW, bool STREAM>
+__global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
     typedef Geo<HD> G;
     typedef typename PagedType<TYPE>::Io Io;
-    constexpr int KW = narrow_waves<HD>(), KEYS = kNarrowKeys, KB = KEYS / 16;
+    constexpr int KEYS = kNarrowKeys, KB = KEYS / 16;
     constexpr int LPW = 2 * KB * G::PPB;  // loads per tile
     constexpr int QB = HD * (int)sizeof(Io), QP = 16 * QB / 1024;  // bytes of a q row, 1 KB loads of 16 of them
     constexpr int D4 = HD / 4;
@@ -884,9 +871,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
 template <int TYPE, int HD>
 hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     if (narrow_grid) {
-        const dim3 grid((unsigned)narrow_grid), block(64 * narrow_waves<HD>());
-        if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, false>), grid, block, 0, s, a);
+        constexpr int KW = narrow_waves<HD>();
+        const dim3 grid((unsigned)narrow_grid);
+        if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a);
+        else if (a.crowd) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, 2, false>), grid, dim3(128), 0, s, a);
+        else hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -970,6 +959,7 @@ hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q
     a.select = select;
     const long long cols = (long long)b->plan.n_tok * b->p->n_kv * ((b->p->group + 15) / 16);
     const long long grid = captured ? b->shape.narrow_wgs : cols * chosen_parts(a.wgs, (int)cols, select, a.shift);
+    a.crowd = cols >= 2 * a.wgs;
     // chosen pages of single tokens are read once, those of a chunk's tokens by many of them
     const bool stream = b->plan.n_tok == (int)b->plan.seqs.size() && cols * ((long long)select << a.shift) * 4 * b->p->head_dim > kStreamBytes;
     return launch_any(b, a, a, stream, (int)std::min<long long>(grid, 1 << 30), 0, s);

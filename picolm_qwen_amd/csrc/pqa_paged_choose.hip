@@ -35,10 +35,18 @@ struct PagedChoose {
     int* chosen;
     int g, n_kv, shift, select, first, last, qvec;
     int group, stride;  // tokens per workgroup; keys per token in LDS
+    int parts;          // workgroups that share a column's pages (group 1)
+    uint32_t* part_keys;  // [column][stride]
+    unsigned* counters;
 };
 
-constexpr int kChooseThreads = 512, kChooseWaves = kChooseThreads / 64;
+// Threads: 1024 for single tokens, whose few workgroups wait for loads; 512 where tokens share one, and at
+// head sizes whose operands need the registers.
+template <int HD>
+constexpr int choose_threads() { return HD <= 128 ? 1024 : 512; }
+constexpr int kChooseWaves = 16;
 constexpr int kWaveKeys = 1024;
+constexpr int kPartPages = 512;  // least pages of a column's part
 constexpr int kChooseBytes = 40 << 10;  // of LDS for the keys, where more than one token shares a workgroup
 
 // 16 elements as whole numbers, rounded to nearest even, of one sign within [lo, hi] and the others as
@@ -64,6 +72,11 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
 
 __device__ __forceinline__ int popcount(unsigned long long x) { return (int)__popcll(x); }
 
+// bits of x below the lane's
+__device__ __forceinline__ int before(unsigned long long x) {
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(x >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)x, 0));
+}
+
 // A token's keys: its forced pages, [0, first) and [p1, n), above all scores.
 struct Keys {
     const uint32_t* k;
@@ -71,39 +84,46 @@ struct Keys {
     __device__ uint32_t operator[](int i) const { return i < first || i >= p1 ? 0xFFFFFFFFu : k[i]; }
 };
 
-// The list of one token by one wave; n <= kWaveKeys.
+// maximum over the wave's lanes, in every lane
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor1, 0xF, 0xF, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor2, 0xF, 0xF, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor7, 0xF, 0xF, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor15, 0xF, 0xF, false));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+
+// The list of one token by one wave, its n <= 64 R keys in registers.
+template <int R>
 __device__ __forceinline__ void choose_by_wave(const Keys& keys, int select, int lane, int* out) {
-    constexpr int R = kWaveKeys / 64;
-    uint32_t k[R];
-    const int regs = (keys.n + 63) / 64;
+    uint32_t k[R], hi = 0, lo = 0;  // lo: of the complements
 #pragma unroll
-    for (int r = 0; r < R; r++) k[r] = r < regs && 64 * r + lane < keys.n ? keys[64 * r + lane] : 0u;
+    for (int r = 0; r < R; r++) {
+        const int i = 64 * r + lane;
+        const uint32_t x = i < keys.n ? keys.k[i] : 0u;
+        const bool score = i >= keys.first && i < keys.p1;
+        if (score) {
+            hi = max(hi, x);
+            lo = max(lo, ~x);
+        }
+        k[r] = i >= keys.n ? 0u : score ? x : 0xFFFFFFFFu;
+    }
+    hi = __builtin_amdgcn_readfirstlane(wave_max(hi));
+    lo = __builtin_amdgcn_readfirstlane(~wave_max(lo));
     auto count = [&](uint32_t least) {
         int c = 0;
 #pragma unroll
-        for (int r = 0; r < R; r++)
-            if (r < regs) c += popcount(__ballot(k[r] >= least));
+        for (int r = 0; r < R; r++) c += popcount(__ballot(k[r] >= least));
         return c;
     };
-    // the bits that all scores share (the forced pages' keys are above them anyway)
-    uint32_t lo = 0xFFFFFFFFu, hi = 0;
-#pragma unroll
-    for (int r = 0; r < R; r++)
-        if (r < regs && 64 * r + lane >= keys.first && 64 * r + lane < keys.p1) {
-            lo = min(lo, k[r]);
-            hi = max(hi, k[r]);
-        }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-        hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    // the largest key that at least `select` keys reach
-    const int top = lo == hi ? -1 : 31 - __clz((int)(lo ^ hi));  // the highest bit in which two scores differ
+    // the largest key that at least `select` keys reach, from the highest bit on in which two scores
+    // differ (the forced pages' keys are above all of them)
+    const int top = lo == hi ? -1 : 31 - __clz((int)(lo ^ hi));
     uint32_t least = top < 0 ? lo : top == 31 ? 0u : lo >> (top + 1) << (top + 1);
-    int reach = count(least);
+    int reach = top == 31 ? keys.n : count(least);
 #pragma unroll 1
     for (int bit = top; bit >= 0 && reach != select; bit--) {
         const uint32_t cand = least | 1u << bit;
@@ -115,15 +135,13 @@ __device__ __forceinline__ void choose_by_wave(const Keys& keys, int select, int
     }
     // above it all, of those that equal it the first `same`
     int same = reach == select ? keys.n : select - (least == 0xFFFFFFFFu ? 0 : count(least + 1)), put = 0;
-    const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        if (r >= regs) break;
         const bool in = 64 * r + lane < keys.n, is = in && k[r] == least;
         const unsigned long long equal = __ballot(is);
-        const bool take = in && (k[r] > least || (is && popcount(equal & below) < same));
+        const bool take = in && (k[r] > least || (is && before(equal) < same));
         const unsigned long long taken = __ballot(take);
-        const int to = put + popcount(taken & below);
+        const int to = put + before(taken);
         if (take && to < select) out[to] = 64 * r + lane;
         put += popcount(taken);
         same = max(0, same - popcount(equal));
@@ -131,21 +149,23 @@ __device__ __forceinline__ void choose_by_wave(const Keys& keys, int select, int
 }
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choose_kernel(const PagedChoose a) {
+__global__ __launch_bounds__(choose_threads<HD>()) void paged_choose_kernel(const PagedChoose a) {
     typedef typename PagedType<TYPE>::Io Io;
     constexpr int ST = HD / 32;              // steps of 64 products
     constexpr int PB = HD <= 128 ? 4 : 2;    // blocks of 16 pages at a time
     extern __shared__ uint32_t lds_keys[];
     __shared__ int hist[256];
     __shared__ uint32_t s_lo[kChooseWaves], s_hi[kChooseWaves];
-    __shared__ int s_digit, s_left, s_gt[kChooseWaves], s_eq[kChooseWaves];
+    __shared__ int s_flag, s_digit, s_left, s_gt[kChooseWaves], s_eq[kChooseWaves];
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g16 = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), threads = blockDim.x, waves = threads >> 6;
     // the tokens whose number is a multiple of the group come first, in one run: most of the others
     // leave at once, and would leave CUs idle in between
     const int n_tok = scalar_int(a.header, kHdTokens), heads = (n_tok + a.group - 1) / a.group;
-    for (int u = blockIdx.x; u < heads * a.group * a.n_kv; u += gridDim.x) {
-        const int kvh = u % a.n_kv, v = u / a.n_kv, tok = v % heads * a.group + v / heads;
+    for (int u = blockIdx.x; u < heads * a.group * a.n_kv * a.parts; u += gridDim.x) {
+        // a column's parts lie next to each other, so on different dies
+        const int col = u / a.parts, part = u - col * a.parts;
+        const int kvh = col % a.n_kv, v = col / a.n_kv, tok = v % heads * a.group + v / heads;
         if (tok >= n_tok) continue;
         const int* token = a.tokens + 4 * (size_t)tok;
         const int table = scalar_int(token, 0), pos = scalar_int(token, 1);
@@ -153,14 +173,22 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
         const int nt = min(a.group, scalar_int(token, 3));
         const int top = ((pos + nt - 1) >> a.shift) + 1;  // pages that the last of the tokens sees
         if (top > a.select) {
-            for (int i = tid; i < nt * a.stride; i += kChooseThreads) lds_keys[i] = 0u;
-            __syncthreads();
-            // scores of pages [p0, p1); 16 columns: heads of the tokens, or 16 heads at a time
-            const int p0 = a.first, p1 = top - a.last;
+            bool ready = false;
+            // scores of pages [p0, p1), of this part's; 16 columns: heads of the tokens, or 16 heads at a time
+            const int all0 = a.first, all1 = top - a.last;
+            const int p0 = all0 + (int)((long long)(all1 - all0) * part / a.parts);
+            const int p1 = all0 + (int)((long long)(all1 - all0) * (part + 1) / a.parts);
             for (int h0 = 0; h0 < a.g; h0 += 16) {
                 const int t = a.g > 16 ? 0 : c16 / a.g, h = a.g > 16 ? h0 + c16 : c16 - t * a.g;
                 const bool column = t < nt && h < a.g;  // the others repeat column 0
                 const Io* q = (const Io*)a.q + (long long)(column ? tok + t : tok) * a.ldq + (long long)(kvh * a.g + (column ? h : 0)) * HD;
+                int page[PB];
+                auto look = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int b = 0; b < PB; b++) page[b] = a.pages[table + min(b0 + 16 * b + c16, all1 - 1)];
+                };
+                int b0 = p0 + 16 * PB * w;
+                if (b0 < p1) look(b0);
                 float x[ST][16], mx = 0.0f;
 #pragma unroll
                 for (int st = 0; st < ST; st++)
@@ -172,6 +200,11 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
                         x[st][4 * i + 2] = y.z;
                         x[st][4 * i + 3] = y.w;
                     }
+                if (!ready) {  // the keys start below all scores; q's loads are on their way meanwhile
+                    for (int i = tid; i < nt * a.stride; i += threads) lds_keys[i] = 0u;
+                    __syncthreads();
+                    ready = true;
+                }
 #pragma unroll
                 for (int st = 0; st < ST; st++)
 #pragma unroll
@@ -185,14 +218,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
                     qb[st] = signed_bytes(x[st], up, neg ? -127.0f : 0.0f, neg ? 0.0f : 127.0f);
                 }
                 uint32_t* mine = lds_keys + (column ? t : 0) * a.stride;
-                int page[PB];
-                auto look = [&](int b0) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int b = 0; b < PB; b++) page[b] = a.pages[table + min(b0 + 16 * b + c16, p1 - 1)];
-                };
-                int b0 = p0 + 16 * PB * w;
-                if (b0 < p1) look(b0);
-                for (; b0 < p1; b0 += 16 * PB * kChooseWaves) {
+                for (; b0 < p1; b0 += 16 * PB * waves) {
                     intx4 y[PB][ST];
                     float sc[PB];
 #pragma unroll
@@ -203,7 +229,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
                         for (int st = 0; st < ST; st++) y[b][st] = *(const intx4*)(r + 64 * st);
                         sc[b] = a.scales[at];  // of page b0 + 16 b + c16
                     }
-                    if (b0 + 16 * PB * kChooseWaves < p1) look(b0 + 16 * PB * kChooseWaves);
+                    if (b0 + 16 * PB * waves < p1) look(b0 + 16 * PB * waves);
 #pragma unroll
                     for (int b = 0; b < PB; b++) {
                         intx4 acc = {0, 0, 0, 0};
@@ -219,17 +245,34 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
                 }
             }
             __syncthreads();
+            if (a.parts > 1) {
+                uint32_t* to = a.part_keys + (size_t)col * a.stride;
+                for (int i = p0 + tid; i < p1; i += threads)
+                    __hip_atomic_store(to + i, lds_keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const bool last = last_of(a.counters + col, a.parts, &s_flag);
+                if (last)
+                    for (int i = all0 + tid; i < all1; i += threads)
+                        lds_keys[i] = __hip_atomic_load(to + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                if (!last) continue;
+            }
+        } else if (part) {
+            continue;
         }
         // a list per token: short ones a wave each
         for (int t = 0; t < nt; t++) {
             const int n = ((pos + t) >> a.shift) + 1;
             if (n > a.select && n > kWaveKeys) continue;
-            if (t % kChooseWaves != w) continue;
+            if (t % waves != w) continue;
             int* out = a.chosen + ((size_t)(tok + t) * a.n_kv + kvh) * a.select;
             if (n <= a.select) {  // every page
                 for (int i = lane; i < a.select; i += 64) out[i] = i < n ? i : -1;
             } else {
-                choose_by_wave(Keys{lds_keys + t * a.stride, a.first, n - a.last, n}, a.select, lane, out);
+                const Keys keys = {lds_keys + t * a.stride, a.first, n - a.last, n};
+                if (n <= 256) choose_by_wave<4>(keys, a.select, lane, out);
+                else if (n <= 512) choose_by_wave<8>(keys, a.select, lane, out);
+                else if (n <= 768) choose_by_wave<12>(keys, a.select, lane, out);
+                else choose_by_wave<16>(keys, a.select, lane, out);
             }
         }
         for (int t = 0; t < nt; t++) {
@@ -240,7 +283,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
             const int p0 = a.first, p1 = n - a.last;
             // the range of the scores, so that the first digit tells them apart
             uint32_t lo = 0xFFFFFFFFu, hi = 0;
-            for (int i = p0 + tid; i < p1; i += kChooseThreads) {
+            for (int i = p0 + tid; i < p1; i += threads) {
                 lo = min(lo, keys.k[i]);
                 hi = max(hi, keys.k[i]);
             }
@@ -255,7 +298,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kChooseWaves; i++) {
+            for (int i = 0; i < waves; i++) {
                 lo = min(lo, s_lo[i]);
                 hi = max(hi, s_hi[i]);
             }
@@ -270,7 +313,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
                     const int width = min(8, shift), next = shift - width;
                     if (tid < 256) hist[tid] = 0;
                     __syncthreads();
-                    for (int i = p0 + tid; i < p1; i += kChooseThreads) {
+                    for (int i = p0 + tid; i < p1; i += threads) {
                         const uint32_t k = keys.k[i] - lo;
                         if (shift >= 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> next) & ((1u << width) - 1)], 1);
                     }
@@ -303,7 +346,7 @@ __global__ __launch_bounds__(kChooseThreads, HD <= 128 ? 4 : 2) void paged_choos
             // keys above lo + prefix are chosen, and the first `left` that equal it (left == 0: the
             // forced pages alone); each wave lists a run of the pages behind what the waves before it found
             const uint32_t at = left > 0 ? lo + prefix : 0xFFFFFFFEu;
-            const int run = (n + kChooseWaves * 64 - 1) / (kChooseWaves * 64) * 64, r0 = w * run, r1 = min(n, r0 + run);
+            const int run = (n + waves * 64 - 1) / (waves * 64) * 64, r0 = w * run, r1 = min(n, r0 + run);
             int gt = 0, eq = 0;
             for (int i = r0 + lane; i < r1; i += 64) {
                 const uint32_t k = keys[i];
@@ -350,7 +393,7 @@ hipError_t launch_choose(const PagedChoose& a, unsigned grid, size_t lds, hipStr
                                                  (kPagedMaxChoice + 1) * 4);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((paged_choose_kernel<TYPE, HD>), dim3(grid), dim3(kChooseThreads), lds, s, a);
+    hipLaunchKernelGGL((paged_choose_kernel<TYPE, HD>), dim3(grid), dim3(a.group > 1 ? 512 : choose_threads<HD>()), lds, s, a);
     return hipGetLastError();
 }
 
@@ -394,9 +437,17 @@ hipError_t launch_paged_choose(const pqa_batch* b, int layer, const PagedRows& q
     if (longest > kPagedMaxChoice) return hipErrorInvalidValue;
     a.stride = longest | 1;  // odd: the tokens' keys of one page lie in different banks
     a.group = std::max(1, std::min(a.g > 16 ? 1 : 16 / a.g, kChooseBytes / (4 * a.stride)));
+    // Few columns share out many pages: one CU's loads take longer than passing the keys on does, some 3 us.
+    const long long columns = (long long)(captured ? b->shape.max_tokens : b->plan.n_tok) * p->n_kv;
+    const long long room = columns ? p->cu_count / columns : 1;
+    a.parts = a.group > 1 && !captured && b->plan.n_tok > (int)b->plan.seqs.size() ? 1 : (int)std::max<long long>(1, std::min<long long>(room, longest / kPartPages));
+    if (a.parts > 1 && columns * a.stride > (long long)pqa::paged_narrow_slots(b->shape) * 16 * (p->head_dim + 2)) a.parts = 1;
+    if (a.parts > 1) a.group = 1;
+    a.part_keys = (uint32_t*)b->part_narrow;
+    a.counters = b->counters;
     const size_t lds = (size_t)a.group * a.stride * 4;
     const long long most = 16LL * p->cu_count;
-    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(1 << 30, ((long long)b->plan.n_tok + a.group) * p->n_kv));
+    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(1 << 30, ((long long)b->plan.n_tok + a.group) * p->n_kv * a.parts));
     switch (p->type) {
         case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(p->head_dim, a, grid, lds, s);
         case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(p->head_dim, a, grid, lds, s);

@@ -40,22 +40,24 @@ __device__ __forceinline__ float from_page(uint16_t x) {
     return (float)__builtin_bit_cast(Page, x);
 }
 
-// four elements of a row as fp32; `vec`: the row's start is aligned to four elements
-template <class Io>
+// four elements of a row as fp32; `vec`: the row's start is aligned to four elements. ONCE: past
+// the caches
+template <class Io, bool ONCE = false>
 __device__ __forceinline__ float4 load4(const Io* p, bool vec) {
     typedef Io v4 __attribute__((ext_vector_type(4)));
     if (vec) {
-        const v4 x = *(const v4*)p;
+        const v4 x = ONCE ? __builtin_nontemporal_load((const v4*)p) : *(const v4*)p;
         return float4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
     }
     return float4{(float)p[0], (float)p[1], (float)p[2], (float)p[3]};
 }
-template <class Io>
+template <class Io, bool ONCE = false>
 __device__ __forceinline__ void store4(Io* p, float4 x, bool vec) {
     typedef Io v4 __attribute__((ext_vector_type(4)));
     const v4 y = {(Io)x.x, (Io)x.y, (Io)x.z, (Io)x.w};
     if (vec) {
-        *(v4*)p = y;
+        if constexpr (ONCE) __builtin_nontemporal_store(y, (v4*)p);
+        else *(v4*)p = y;
         return;
     }
 #pragma unroll
@@ -73,6 +75,22 @@ __device__ __forceinline__ float power2(int e) { return __uint_as_float((unsigne
 __device__ __forceinline__ void lds_dma_b128_at(const void* p, unsigned lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+}
+
+// Called by the whole workgroup after its part's stores (agent scope, relaxed: past the L2s, which are
+// not coherent between dies); true in the workgroup that finishes last, which then sees all
+// parts. Its counter is zero again for the next call.
+__device__ __forceinline__ bool last_of(unsigned* counter, int parts, int* flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have reached memory
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = n == (unsigned)parts - 1;
+        if (*flag) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    asm volatile("" ::: "memory");  // the loads of the parts stay behind the counter
+    return *flag != 0;
 }
 
 // a table that the kernel only reads, through the scalar cache
