@@ -81,9 +81,7 @@ hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q
                                hipStream_t s);
 // most pages of one sequence that a choice can be made of: their scores fit the LDS
 constexpr int kPagedMaxChoice = 32768;
-hipError_t launch_paged_choose(const pqa_batch* b, int layer, const PagedRows& q, int select, int first, int last, int* chosen,
-                               bool captured, hipStream_t s);
-hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q, int select, const int* chosen, void* out,
-                               long long ldo, bool captured, hipStream_t s);
+hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q, int select, int first, int last, int* chosen,
+                               void* out, long long ldo, bool captured, hipStream_t s);
 
 }  // namespace pqa

@@ -513,9 +513,8 @@ extern "C" int pqa_paged_attend_sparse(pqa_paged* p, pqa_batch* b, int layer, co
             return fail(p, PQA_ERR_UNSUPPORTED, name + ": more than " + std::to_string(pqa::kPagedMaxChoice) +
                                                     " pages in a sequence" + (captured ? " (captured: the batch's most)" : ""));
         const pqa::PagedRows rows = {q, q_stride};
-        hipError_t e = pqa::launch_paged_choose(b, layer, rows, select, first, last, chosen, captured, (hipStream_t)stream);
-        if (e == hipSuccess)
-            e = pqa::launch_paged_chosen(b, layer, rows, select, chosen, out, out_stride, captured, (hipStream_t)stream);
+        const hipError_t e =
+            pqa::launch_paged_sparse(b, layer, rows, select, first, last, chosen, out, out_stride, captured, (hipStream_t)stream);
         return e == hipSuccess ? PQA_OK : hip_fail(p, e, name);
     });
 }

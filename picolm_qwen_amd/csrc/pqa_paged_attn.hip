@@ -9,9 +9,11 @@
 // global->LDS loads, 16-byte chunk c of row r at slot c ^ x(r), which keeps the K operand reads
 // and the transposing V reads free of bank conflicts.
 //
-// Types: fp16 and bf16 rows enter the products as they are, P is rounded to the same type
-// (half a step, 2^-11 or 2^-8 of a weight; errors of many weights average out, and the output
-// is rounded to that type anyway). fp32 rows are split into two fp16 parts with 22
+// Types: fp16 and bf16 rows enter the products as they are. P is rounded to the same type in the wide
+// kernel (half a step, 2^-11 or 2^-8 of a weight, which leaves at most as much error as the output's
+// own rounding; a second product would cost a third of its time), and split into a high and a low part in the narrow
+// one, where products are free (not by the workgroups of two waves, which a chunk's chosen pages feed
+// from the caches: 191 us with it, 178 without, for 300 tokens). fp32 rows are split into two fp16 parts with 22
 // significant bits together (after an exact power of two), and so is P, the low parts' sums
 // apart: fp32-level results at twice the products. Scores, maxima and sums are fp32 throughout.
 //
@@ -30,7 +32,7 @@
 // slow_rows, in fp32 over its own keys alone.
 #include <algorithm>
 
-#include "pqa_paged_device.h"
+#include "pqa_paged_choose.h"
 
 namespace pqa {
 
@@ -64,8 +66,9 @@ struct PagedAttn {
 // rows and keys of one piece of work
 struct Column {
     int row0, rows, hist, table, kvh, r0;
-    int kend;         // keys that exist
-    const int* list;  // its chosen pages, or null: all pages of the sequence
+    int kend;          // keys that exist
+    const int* list;   // its chosen pages, or null: all pages of the sequence
+    const int* local;  // in LDS: ids of the chosen pages themselves, or null
 };
 
 constexpr int pow2_of(int ch) { return ch % 16 == 0 ? 16 : ch % 8 == 0 ? 8 : ch % 4 == 0 ? 4 : ch % 2 == 0 ? 2 : 1; }
@@ -107,6 +110,7 @@ struct Ops<PQA_PAGED_BF16> {
 };
 
 __device__ __forceinline__ int page_at(const PagedAttn& a, const Column& c, int i) {
+    if (c.local) return __builtin_amdgcn_readfirstlane(c.local[i]);
     const int j = c.list ? scalar_int(c.list, i) : i;
     return scalar_int(a.pages, c.table + j);
 }
@@ -193,8 +197,8 @@ struct RowBlock {
 };
 
 // One tile of KEYS keys from key0 on for RB row blocks. kl and vl: the tile in LDS. masked:
-// some row of the wave ends inside the tile.
-template <int TYPE, int HD, int KEYS, int RB>
+// some row of the wave ends inside the tile. LOW: P's low part of 16-bit rows as well.
+template <int TYPE, int HD, int KEYS, int RB, bool LOW>
 __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const char* kl, const char* vl, int key0, bool masked,
                                           const int (&koff)[Geo<HD>::KS], const int (&voff)[Geo<HD>::DB], int g16) {
     typedef Ops<TYPE> O;
@@ -223,7 +227,8 @@ __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const ch
         }
     }
     // keys key0 + 16 kb + 4 g16 + e of row c16
-    V8 ph[RB][KB / 2], pl[O::split ? RB : 1][KB / 2];
+    constexpr bool low = O::split || LOW;
+    V8 ph[RB][KB / 2], pl[low ? RB : 1][KB / 2];
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         RowBlock<TYPE, HD>& b = rb[r];
@@ -261,9 +266,10 @@ __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const ch
                 float p = fast_exp2(fmaf(s[r][kb][e], b.cs, -mc));
                 if constexpr (O::split) p *= O::scale;
                 b.l += p;
-                ph[r][kb >> 1][4 * (kb & 1) + e] = (typename PagedType<TYPE>::Page)p;
-                if constexpr (O::split)
-                    pl[r][kb >> 1][4 * (kb & 1) + e] = (_Float16)((p - (float)ph[r][kb >> 1][4 * (kb & 1) + e]) * kLow);
+                const auto hi = (typename PagedType<TYPE>::Page)p;
+                ph[r][kb >> 1][4 * (kb & 1) + e] = hi;
+                if constexpr (low)
+                    pl[r][kb >> 1][4 * (kb & 1) + e] = (typename PagedType<TYPE>::Page)((p - (float)hi) * (O::split ? kLow : 1.0f));
             }
     }
 #pragma unroll
@@ -282,6 +288,7 @@ __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const ch
             for (int r = 0; r < RB; r++) {
                 rb[r].o[db] = O::mul(vf, ph[r][h], rb[r].o[db]);
                 if constexpr (O::split) rb[r].ol[db] = O::mul(vf, pl[r][h], rb[r].ol[db]);
+                else if constexpr (LOW) rb[r].o[db] = O::mul(vf, pl[r][h], rb[r].o[db]);
             }
         }
 }
@@ -322,7 +329,7 @@ __device__ __forceinline__ void slow_rows(const PagedAttn& a, const Column& c, f
         const bool in = tile < end && key <= qlast;
         const int at = in ? key : kt * KEYS;  // some key that exists
         const int pi = at >> a.shift;
-        const int page = a.pages[c.table + (c.list ? c.list[pi] : pi)];
+        const int page = c.local ? c.local[pi] : a.pages[c.table + (c.list ? c.list[pi] : pi)];
         // within a layer's rows, which fit 31 bits
         const int krow = (int)((((unsigned)page * a.n_kv + c.kvh) << a.shift) + (at & ((1 << a.shift) - 1)));
         const u32x4* kr = (const u32x4*)(a.kp + (size_t)krow * Geo<HD>::ROWB);
@@ -538,12 +545,16 @@ __host__ __device__ inline int chosen_parts(int wgs, int cols, int select, int s
     return (int)(room < 1 ? 1 : room < most ? room : most);
 }
 
-template <int HD>
-constexpr int narrow_waves() { return HD <= 128 ? 4 : 2; }
+constexpr int narrow_waves(int hd) { return hd <= 128 ? 4 : 2; }
 
-// ---- up to 16 rows: waves on different key tiles ----
-template <int TYPE, int HD, int KW, bool STREAM>
-__global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
+// Chosen pages of a column that one workgroup can hold besides its tiles.
+constexpr int kFusedPages = 2048;
+
+// ---- up to 16 rows: waves on different key tiles. CHOOSE: the workgroup makes the choice of its column's
+// pages first, for single tokens: no second launch, and no column waits for the one with the most
+// pages (32 tokens of 32 / 8 heads of 128, 32 of 125 to 886 pages each: 67.7 us in two launches, 57.9) ----
+template <int TYPE, int HD, int KW, bool STREAM, bool CHOOSE>
+__device__ __forceinline__ void narrow_body(const PagedAttn& a, const PagedChoose* ch) {
     typedef Geo<HD> G;
     typedef typename PagedType<TYPE>::Io Io;
     constexpr int KEYS = kNarrowKeys, KB = KEYS / 16;
@@ -554,6 +565,7 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_na
     __shared__ __attribute__((aligned(1024))) char sq[16 * QB];
     __shared__ float s_ml[KW][2][16];
     __shared__ int s_flag;
+    __shared__ int s_page[CHOOSE ? kFusedPages : 1];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -610,7 +622,37 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_na
             c.table = scalar_int(a.tokens, 4 * tok);
             c.kvh = tk - tok * a.n_kv;
             c.r0 = 16 * blk;
-            c.list = a.chosen + (size_t)tk * a.select;
+            c.list = CHOOSE ? nullptr : a.chosen + (size_t)tk * a.select;
+            c.local = nullptr;
+            if constexpr (CHOOSE) {
+                __shared__ ListScratch scratch;
+                const int n = (pos >> a.shift) + 1;
+                if (n > a.select) {
+                    uint32_t* room = (uint32_t*)&lds[0][0][0][0];
+                    score_pages<TYPE, HD, (HD <= 128 ? 8 : 4)>(*ch, room, tok, 1, c.kvh, c.table, ch->first, n - ch->last, w, KW);
+                    __syncthreads();
+                    const Keys keys = {room, ch->first, n - ch->last, n};
+                    if (n > kWaveKeys) choose_by_block(keys, a.select, scratch, w, KW, s_page);
+                    else if (w == 0) {
+                        if (n <= 256) choose_by_wave<4>(keys, a.select, lane, s_page);
+                        else if (n <= 512) choose_by_wave<8>(keys, a.select, lane, s_page);
+                        else if (n <= 768) choose_by_wave<12>(keys, a.select, lane, s_page);
+                        else choose_by_wave<16>(keys, a.select, lane, s_page);
+                    }
+                } else {
+                    for (int i = tid; i < n; i += 64 * KW) s_page[i] = i;
+                }
+                __syncthreads();
+                int* out = ch->chosen + (size_t)tk * a.select;
+                for (int i = tid; i < a.select; i += 64 * KW) {
+                    const int p = i < seen ? s_page[i] : -1;
+                    if (part == 0 && blk == 0) out[i] = p;
+                    if (p >= 0) s_page[i] = a.pages[c.table + p];
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no store among the counted loads
+                __syncthreads();
+                c.local = s_page;
+            }
             const int tiles = (c.kend + KEYS - 1) / KEYS;
             t0 = (int)((long long)tiles * part / parts);
             t1 = (int)((long long)tiles * (part + 1) / parts);
@@ -633,6 +675,7 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_na
             counter = scalar_int(p, 11);
             c.kend = c.hist + (c.rows - 1) / a.g + 1;
             c.list = nullptr;
+            c.local = nullptr;
         }
         const int nrow = min(16, c.rows - c.r0);
         const int tile0 = t0 + w;  // this wave's tiles: tile0, tile0 + KW, ...
@@ -697,7 +740,7 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_na
         for (int kt = tile0; kt < t1; kt += KW) {
             if (kt + KW < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPW < 63 ? LPW : 63) : "memory");  // the next tile's stay in flight
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            tile_step<TYPE, HD, KEYS, 1>(rb, lds[w][buf][0], lds[w][buf][1], kt * KEYS, kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
+            tile_step<TYPE, HD, KEYS, 1, KW == narrow_waves(HD)>(rb, lds[w][buf][0], lds[w][buf][1], kt * KEYS, kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer has been read
             issue(kt + 2 * KW, buf);
             buf ^= 1;
@@ -738,6 +781,16 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_na
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no store among the next item's counted loads
         __syncthreads();  // LDS is free again
     }
+}
+
+template <int TYPE, int HD, int KW, bool STREAM>
+__global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_narrow_kernel(const PagedAttn a) {
+    narrow_body<TYPE, HD, KW, STREAM, false>(a, nullptr);
+}
+
+template <int TYPE, int HD, int KW, bool STREAM>
+__global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_sparse_kernel(const PagedAttn a, const PagedChoose ch) {
+    narrow_body<TYPE, HD, KW, STREAM, true>(a, &ch);
 }
 
 template <int TYPE, int HD>
@@ -795,6 +848,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
                   parts = scalar_int(p, 10), counter = scalar_int(p, 11);
         c.kend = c.hist + (c.rows - 1) / a.g + 1;
         c.list = nullptr;
+        c.local = nullptr;
 
         int page;  // of the wave's block in the tile that is loaded next
         auto look = [&](int kt) __attribute__((always_inline)) {
@@ -838,7 +892,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
             __syncthreads();                                   // everyone's; the other buffer is free
             issue(kt + 1, buf ^ 1);
             if (kt * KEYS <= qmax)
-                tile_step<TYPE, HD, KEYS, RB>(rb, lds + 2 * buf * TILE, lds + (2 * buf + 1) * TILE, kt * KEYS,
+                tile_step<TYPE, HD, KEYS, RB, false>(rb, lds + 2 * buf * TILE, lds + (2 * buf + 1) * TILE, kt * KEYS,
                                               kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
             buf ^= 1;
         }
@@ -869,11 +923,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
 }
 
 template <int TYPE, int HD>
-hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     if (narrow_grid) {
-        constexpr int KW = narrow_waves<HD>();
+        constexpr int KW = narrow_waves(HD);
         const dim3 grid((unsigned)narrow_grid);
-        if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a);
+        if (ch) {
+            if (stream) hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a, *ch);
+            else hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a, *ch);
+        } else if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a);
         else if (a.crowd) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, 2, false>), grid, dim3(128), 0, s, a);
         else hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a);
         const hipError_t e = hipGetLastError();
@@ -887,20 +944,20 @@ hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, bool stream
 }
 
 template <int TYPE>
-hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (hd) {
-#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, stream, narrow_grid, wide_grid, s);
+#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, ch, stream, narrow_grid, wide_grid, s);
         PQA_PG(64) PQA_PG(96) PQA_PG(128) PQA_PG(160) PQA_PG(192) PQA_PG(256)
 #undef PQA_PG
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (b->p->type) {
-        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
-        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
-        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, stream, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
+        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
     }
 }
 
@@ -949,20 +1006,30 @@ hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q
     // any content fits
     const int n = captured ? b->shape.narrow_wgs : (int)b->plan.runs.size();
     const int w = captured ? b->shape.wide_wgs : (int)b->plan.wide.size();
-    return launch_any(b, a, wide, b->plan.stream, n, w, s);
+    return launch_any(b, a, wide, nullptr, b->plan.stream, n, w, s);
 }
 
-hipError_t launch_paged_chosen(const pqa_batch* b, int layer, const PagedRows& q, int select, const int* chosen, void* out,
-                               long long ldo, bool captured, hipStream_t s) {
+hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q, int select, int first, int last, int* chosen,
+                               void* out, long long ldo, bool captured, hipStream_t s) {
+    const pqa_paged* p = b->p;
     PagedAttn a = arguments(b, layer, q, out, ldo);
     a.chosen = chosen;
     a.select = select;
-    const long long cols = (long long)b->plan.n_tok * b->p->n_kv * ((b->p->group + 15) / 16);
+    PagedChoose ch = choose_arguments(b, layer, q, select, first, last, chosen, captured);
+    const long long cols = (long long)b->plan.n_tok * p->n_kv * ((p->group + 15) / 16);
     const long long grid = captured ? b->shape.narrow_wgs : cols * chosen_parts(a.wgs, (int)cols, select, a.shift);
-    a.crowd = cols >= 2 * a.wgs;
+    // tokens of one sequence share the loads of a choice, and long columns its work: a launch of its own for these
+    const bool tokens = captured ? b->shape.max_tokens <= b->shape.max_seqs : ch.single;
+    const bool fused = tokens && ch.parts == 1 && select <= kFusedPages &&
+                       4 * ch.stride <= narrow_waves(p->head_dim) * 2 * kNarrowKeys * 4 * p->head_dim;
+    if (!fused) {
+        const hipError_t e = launch_paged_choose(b, ch, captured, s);
+        if (e != hipSuccess) return e;
+    }
+    a.crowd = !fused && cols >= 2 * a.wgs;
     // chosen pages of single tokens are read once, those of a chunk's tokens by many of them
-    const bool stream = b->plan.n_tok == (int)b->plan.seqs.size() && cols * ((long long)select << a.shift) * 4 * b->p->head_dim > kStreamBytes;
-    return launch_any(b, a, a, stream, (int)std::min<long long>(grid, 1 << 30), 0, s);
+    const bool stream = ch.single && cols * ((long long)select << a.shift) * 4 * p->head_dim > kStreamBytes;
+    return launch_any(b, a, a, fused ? &ch : nullptr, stream, (int)std::min<long long>(grid, 1 << 30), 0, s);
 }
 
 }  // namespace pqa
