@@ -59,13 +59,14 @@ struct pqa_batch {
 namespace pqa {
 
 // what the kernels read of a batch, so that a captured call follows the batch's later sets
-enum : int { kHdTokens = 0, kHdTouched = 1, kHdRuns = 2, kHdWide = 3, kPagedHeader = 4 };
+enum : int { kHdTokens = 0, kHdTouched = 1, kHdRuns = 2, kHdWide = 3, kHdSmall = 4, kPagedHeader = 8 };
 
 inline bool paged_head_dim(int hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 160 || hd == 192 || hd == 256; }
 inline int paged_io_bytes(int type) { return type == PQA_PAGED_F32 ? 4 : 2; }
 
 // the attention kernels' tiles (pqa_paged_attn.hip)
 int paged_wide_rows(int type, int hd);
+int paged_least_rows();
 int paged_wide_keys(int hd);
 int paged_narrow_wgs(int hd, int cu_count);
 int paged_wide_wgs(int hd, int cu_count);

@@ -268,6 +268,7 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
         s.narrow_wgs = pqa::paged_narrow_wgs(p->head_dim, p->cu_count);
         s.wide_wgs = pqa::paged_wide_wgs(p->head_dim, p->cu_count);
         s.wide_rows = pqa::paged_wide_rows(p->type, p->head_dim);
+        s.least_rows = pqa::paged_least_rows();
         s.wide_keys = pqa::paged_wide_keys(p->head_dim);
         s.key_bytes = 4 * p->head_dim;
         s.max_seqs = max_seqs;
@@ -275,11 +276,11 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
         s.max_seq_pages = (int)(((long long)max_len + p->page_size - 1) / p->page_size);
         b->max_touched = std::min<size_t>((size_t)max_tokens, (size_t)2 * max_seqs + max_tokens / p->page_size);
         b->max_rest = (size_t)max_seqs * p->n_kv + s.narrow_wgs;
-        // blocks of every sequence, and as many parts again
-        b->max_wide = ((size_t)max_tokens * p->group / s.wide_rows + max_seqs) * p->n_kv + 2 * s.wide_wgs;
+        // blocks of every sequence (up to two of least_rows each, while these are fewer than wide_wgs), and their parts
+        b->max_wide = ((size_t)max_tokens * p->group / s.wide_rows + max_seqs) * p->n_kv + 4 * s.wide_wgs;
         const size_t entries = (size_t)max_seqs * s.max_seq_pages;
         // no plan of this capacity leaves more partials: a block of rows is cut into at most max_len / kWideLeast + 1 parts
-        const size_t blocks = (size_t)max_tokens * p->group <= pqa::kNarrowRows ? 0 : (size_t)max_tokens * p->group / s.wide_rows + std::min(max_seqs, max_tokens);
+        const size_t blocks = (size_t)max_tokens * p->group <= pqa::kNarrowRows ? 0 : (size_t)max_tokens * p->group / s.least_rows + std::min(max_seqs, max_tokens);
         const size_t wide_parts = std::min<size_t>(pqa::paged_wide_slots(s), blocks * p->n_kv * ((size_t)max_len / pqa::kWideLeast + 1));
         struct {
             void** p;
@@ -346,7 +347,9 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         if (e == hipSuccess) e = is_captured(st, &captured);
         if (e != hipSuccess) return hip_fail(p, e, name);
         if (captured) return fail(p, PQA_ERR_ARG, name + ": not while the stream is captured (replayed calls follow a later set)");
-        const int header[pqa::kPagedHeader] = {plan.n_tok, (int)plan.touched.size(), (int)plan.runs.size(), (int)plan.wide.size()};
+        const bool small = plan.wide_rows < s.wide_rows;
+        const int header[pqa::kPagedHeader] = {plan.n_tok, (int)plan.touched.size(), (int)plan.runs.size(),
+                                               small ? 0 : (int)plan.wide.size(), small ? (int)plan.wide.size() : 0};
         const struct {
             void* dst;
             const void* src;

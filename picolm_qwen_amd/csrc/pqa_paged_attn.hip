@@ -480,57 +480,95 @@ __device__ __forceinline__ float2 part_load2(const float* p) {
 }
 
 // Joins the parts of `rows` rows in the order of the parts. lds: BYTES of the workgroup's LDS; the
-// rows go in groups whose maxima and sums fit it. Where a group has fewer elements
-// than the workgroup threads, several threads share an element's parts.
+// rows go in groups whose maxima and sums fit it. What costs time is the latency of the loads, so
+// that 8 of a thread are on their way at once: of two elements of the rows where a group has more than the
+// workgroup threads, else of one element's parts, which then several threads share. (16 took registers
+// from the products: the wide kernel spilled.)
 template <int TYPE, int HD, int ROWS, int BYTES>
 __device__ __forceinline__ void join_parts(const PagedAttn& a, const Column& c, int slot0, int parts, int rows, char* lds) {
-    constexpr int D4 = HD / 4;
+    constexpr int D4 = HD / 4, T = 2, U = 4;
     constexpr size_t F = Slots<HD, ROWS>::FLOATS;
     const float* base = a.part + (size_t)slot0 * F;
     const int tid = threadIdx.x, nt = blockDim.x;
-    floatx4* s_a = (floatx4*)lds;                 // [threads]
-    float2* s_w = (float2*)(lds + 16 * 256);      // [rows of a group][parts]: weight and sum
-    const int fit = (BYTES - 16 * 256) / (8 * parts), step = min(rows, max(1, fit));
+    floatx4* s_a = (floatx4*)lds;                          // [threads]
+    float* s_l = (float*)(lds + 16 * 256);                 // [ROWS] sums of all parts
+    float2* s_w = (float2*)(lds + 16 * 256 + 4 * ROWS);    // [rows of a group][parts]: maximum (then weight) and sum
+    const int fit = (BYTES - 16 * 256 - 4 * ROWS) / (8 * parts), step = min(rows, max(1, fit));
     for (int g0 = 0; g0 < rows; g0 += step) {
         const int n = min(step, rows - g0);
+#pragma unroll 2
         for (int i = tid; i < n * parts; i += nt) {
             const int p = i / n, r = i - p * n;
             s_w[r * parts + p] = part_load2(base + p * F + ROWS * HD + 2 * (g0 + r));
         }
         __syncthreads();
-        const int tasks = n * D4, share = max(1, min(parts, nt / tasks));
-        for (int i0 = 0; i0 < tasks * share; i0 += nt) {
-            const int i = i0 + tid, j = i / tasks, t = i - j * tasks, r = t / D4, d = 4 * (t - r * D4);
-            const bool live = i < tasks * share;
+        for (int r = tid; r < n; r += nt) {
+            float2* w = s_w + r * parts;
             float M = kNone, L = 0.0f;
+            bool nan = false;
+            for (int p = 0; p < parts; p++) {
+                nan |= !(w[p].x == w[p].x);
+                M = fmaxf(M, w[p].x);
+            }
+            if (nan) M = __builtin_nanf("");
+            for (int p = 0; p < parts; p++) {
+                const float e = fast_exp2(w[p].x - M);
+                L = fmaf(e, w[p].y, L);
+                w[p].x = e;
+            }
+            s_l[r] = L;
+        }
+        __syncthreads();
+        const int tasks = n * D4, share = max(1, min(parts, nt / tasks));
+        if (share > 1) {
+            const int j = tid / tasks, t = tid - j * tasks, r = t / D4, d = 4 * (t - r * D4);
             floatx4 A = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (live) {
-                const float2* w = s_w + r * parts;
-                bool nan = false;
-                for (int p = 0; p < parts; p++) {
-                    nan |= !(w[p].x == w[p].x);
-                    M = fmaxf(M, w[p].x);
-                }
-                if (nan) M = __builtin_nanf("");
-                for (int p = 0; p < parts; p++) L = fmaf(fast_exp2(w[p].x - M), w[p].y, L);
+            if (j < share) {
                 const float* src = base + (g0 + r) * HD + d;
-                int p = j;
-                for (; p + 7 * share < parts; p += 8 * share) {
-                    floatx4 x[8];
+#pragma unroll 1
+                for (int p0 = j; p0 < parts; p0 += T * U * share) {
+                    floatx4 x[T * U];  // past the last part: that one again, left out below
 #pragma unroll
-                    for (int u = 0; u < 8; u++) x[u] = part_load4(src + (p + u * share) * F);
+                    for (int u = 0; u < T * U; u++) x[u] = part_load4(src + min(p0 + u * share, parts - 1) * F);
 #pragma unroll
-                    for (int u = 0; u < 8; u++) A += fast_exp2(w[p + u * share].x - M) * x[u];
+                    for (int u = 0; u < T * U; u++)
+                        if (p0 + u * share < parts) A += s_w[r * parts + p0 + u * share].x * x[u];
                 }
-                for (; p < parts; p += share) A += fast_exp2(w[p].x - M) * part_load4(src + p * F);
             }
-            if (share > 1) {  // then tasks * share <= threads: one turn
-                s_a[tid] = A;
-                __syncthreads();
-                if (live && j == 0)
-                    for (int u = 1; u < share; u++) A += s_a[tid + u * tasks];
+            s_a[tid] = A;
+            __syncthreads();
+            if (j == 0) {
+                for (int u = 1; u < share; u++) A += s_a[tid + u * tasks];
+                store_out<TYPE, HD>(a, c, c.r0 + g0 + r, d, A, s_l[r]);
             }
-            if (live && j == 0) store_out<TYPE, HD>(a, c, c.r0 + g0 + r, d, A, L);
+        } else {
+#pragma unroll 1
+            for (int i0 = tid; i0 < tasks; i0 += T * nt) {
+                const int i1 = min(i0 + nt, tasks - 1);
+                const float *s0 = base + g0 * HD + 4 * i0, *s1 = base + g0 * HD + 4 * i1;
+                const float2 *w0 = s_w + i0 / D4 * parts, *w1 = s_w + i1 / D4 * parts;
+                floatx4 A0 = {0.0f, 0.0f, 0.0f, 0.0f}, A1 = A0;
+#pragma unroll 1
+                for (int p0 = 0; p0 < parts; p0 += U) {
+                    floatx4 x0[U], x1[U];  // past the last part: that one again, left out below
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const size_t at = min(p0 + u, parts - 1) * F;
+                        x0[u] = part_load4(s0 + at);
+                        x1[u] = part_load4(s1 + at);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        if (p0 + u < parts) {
+                            A0 += w0[p0 + u].x * x0[u];
+                            A1 += w1[p0 + u].x * x1[u];
+                        }
+                }
+                int r = i0 / D4;
+                store_out<TYPE, HD>(a, c, c.r0 + g0 + r, 4 * (i0 - r * D4), A0, s_l[r]);
+                r = i1 / D4;
+                if (i0 + nt < tasks) store_out<TYPE, HD>(a, c, c.r0 + g0 + r, 4 * (i1 - r * D4), A1, s_l[r]);
+            }
         }
         __syncthreads();
     }
@@ -793,17 +831,18 @@ __global__ __launch_bounds__(64 * KW, KW == 4 && HD == 64 ? 2 : 1) void paged_sp
     narrow_body<TYPE, HD, KW, STREAM, true>(a, &ch);
 }
 
-template <int TYPE, int HD>
-constexpr int wide_blocks() { return TYPE != PQA_PAGED_F32 && HD <= 128 ? 2 : 1; }
+// blocks of 16 rows per wave: two share each operand read where the registers hold them; one for batches
+// that would leave CUs idle
+constexpr int wide_blocks(int type, int hd) { return type != PQA_PAGED_F32 && hd <= 128 ? 2 : 1; }
 template <int HD>
 constexpr int wide_keys() { return HD > 192 ? 32 : 64; }
 
 // ---- more rows: 4 waves share each key tile, RB blocks of 16 rows each ----
-template <int TYPE, int HD>
+template <int TYPE, int HD, int RB>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_wide_kernel(const PagedAttn a) {
     typedef Geo<HD> G;
     typedef typename PagedType<TYPE>::Io Io;
-    constexpr int KEYS = wide_keys<HD>(), KB = KEYS / 16, RB = wide_blocks<TYPE, HD>(), ROWS = 64 * RB;
+    constexpr int KEYS = wide_keys<HD>(), KB = KEYS / 16, ROWS = 64 * RB;
     constexpr int D4 = HD / 4;
     constexpr int TILE = KB * G::BLKB;
     constexpr int WAVE = 20 * G::QS * 4;  // a wave's result and its slow rows' q
@@ -834,7 +873,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
             goff[o][i] = r * G::ROWB + 16 * ((L % G::CH) ^ (lo0 + o ? G::xv(r) : G::xk(r)));
         }
 
-    const int n_items = scalar_int(a.header, kHdWide);
+    const int n_items = scalar_int(a.header, RB == wide_blocks(TYPE, HD) ? kHdWide : kHdSmall);
     for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
         const int* p = a.items + (size_t)it * (sizeof(PagedItem) / 4);
         Column c;
@@ -923,7 +962,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
 }
 
 template <int TYPE, int HD>
-hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
     if (narrow_grid) {
         constexpr int KW = narrow_waves(HD);
         const dim3 grid((unsigned)narrow_grid);
@@ -936,28 +975,36 @@ hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const Paged
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (wide_grid) {
-        hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
-        return hipGetLastError();
+    // a captured call launches both tiles; the one that the batch's items are not made for finds none
+    constexpr int RB = wide_blocks(TYPE, HD);
+    if (wide_grid && (captured || !small)) {
+        hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, RB>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
+    if constexpr (RB > 1)
+        if (wide_grid && (captured || small)) {
+            hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, 1>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
+            return hipGetLastError();
+        }
     return hipSuccess;
 }
 
 template <int TYPE>
-hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (hd) {
-#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, ch, stream, narrow_grid, wide_grid, s);
+#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
         PQA_PG(64) PQA_PG(96) PQA_PG(128) PQA_PG(160) PQA_PG(192) PQA_PG(256)
 #undef PQA_PG
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
     switch (b->p->type) {
-        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
-        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
-        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, ch, stream, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
+        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
     }
 }
 
@@ -990,7 +1037,8 @@ PagedAttn arguments(const pqa_batch* b, int layer, const PagedRows& q, void* out
 
 }  // namespace
 
-int paged_wide_rows(int type, int hd) { return type != PQA_PAGED_F32 && hd <= 128 ? 128 : 64; }
+int paged_wide_rows(int type, int hd) { return 64 * wide_blocks(type, hd); }
+int paged_least_rows() { return 64; }
 int paged_wide_keys(int hd) { return hd > 192 ? 32 : 64; }
 int paged_narrow_wgs(int hd, int cu_count) { return hd == 64 ? 2 * cu_count : cu_count; }
 int paged_wide_wgs(int hd, int cu_count) { return hd == 64 ? 3 * cu_count : hd <= 128 ? 2 * cu_count : cu_count; }
@@ -1006,7 +1054,7 @@ hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q
     // any content fits
     const int n = captured ? b->shape.narrow_wgs : (int)b->plan.runs.size();
     const int w = captured ? b->shape.wide_wgs : (int)b->plan.wide.size();
-    return launch_any(b, a, wide, nullptr, b->plan.stream, n, w, s);
+    return launch_any(b, a, wide, nullptr, b->plan.stream, b->plan.wide_rows < b->shape.wide_rows, captured, n, w, s);
 }
 
 hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q, int select, int first, int last, int* chosen,
@@ -1029,7 +1077,7 @@ hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q
     a.crowd = !fused && cols >= 2 * a.wgs;
     // chosen pages of single tokens are read once, those of a chunk's tokens by many of them
     const bool stream = ch.single && cols * ((long long)select << a.shift) * 4 * p->head_dim > kStreamBytes;
-    return launch_any(b, a, a, fused ? &ch : nullptr, stream, (int)std::min<long long>(grid, 1 << 30), 0, s);
+    return launch_any(b, a, a, fused ? &ch : nullptr, stream, false, captured, (int)std::min<long long>(grid, 1 << 30), 0, s);
 }
 
 }  // namespace pqa

@@ -30,6 +30,7 @@ static PagedShape shape(int page, int group, int n_kv, int wgs, int rows, int ke
     s.narrow_wgs = wgs;
     s.wide_wgs = 2 * wgs;
     s.wide_rows = rows;
+    s.least_rows = 64;
     s.wide_keys = keys;
     s.max_seqs = 96;
     s.max_tokens = 8192;
@@ -47,7 +48,7 @@ static PagedShape shape(int page, int group, int n_kv, int wgs, int rows, int ke
     } while (0)
 
 static int check(int trial, const PagedShape& s, const PagedPlan& p, const std::vector<PagedItem>& items, bool wide) {
-    const int rows = wide ? s.wide_rows : kNarrowRows, keys = wide ? s.wide_keys : kNarrowKeys;
+    const int rows = wide ? p.wide_rows : kNarrowRows, keys = wide ? s.wide_keys : kNarrowKeys;
     const int slots = wide ? paged_wide_slots(s) : paged_narrow_slots(s), counters = wide ? s.wide_wgs : s.narrow_wgs;
     std::map<std::tuple<int, int, int>, std::vector<PagedItem>> blocks;
     for (const PagedItem& it : items) blocks[{it.table, it.kvh, it.r0}].push_back(it);
@@ -86,7 +87,7 @@ static int check(int trial, const PagedShape& s, const PagedPlan& p, const std::
             }
     }
     CHECK(want == items.size());
-    const size_t most = wide ? ((size_t)s.max_tokens * s.group / s.wide_rows + s.max_seqs) * s.n_kv + 2 * s.wide_wgs
+    const size_t most = wide ? ((size_t)s.max_tokens * s.group / s.wide_rows + s.max_seqs) * s.n_kv + 4 * s.wide_wgs
                              : (size_t)s.max_seqs * s.n_kv + s.narrow_wgs;
     CHECK(items.size() <= most);
     return 0;
@@ -156,7 +157,7 @@ int main() {
             longest = std::max(longest, len[i]);
             rows = std::max(rows, n_new[i] * s.group);
         }
-        if ((long long)p.n_tok * s.group > kNarrowRows) blocks = (size_t)p.n_tok * s.group / s.wide_rows + std::min(n, p.n_tok);
+        if ((long long)p.n_tok * s.group > kNarrowRows) blocks = (size_t)p.n_tok * s.group / s.least_rows + std::min(n, p.n_tok);
         for (const PagedItem& it : p.wide) cut = std::max(cut, it.parts > 1 ? (size_t)it.slot0 + it.parts : 0);
         CHECK(cut <= blocks * s.n_kv * (longest / kWideLeast + 1));
     }
