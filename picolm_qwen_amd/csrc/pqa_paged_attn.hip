@@ -226,6 +226,9 @@ __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const ch
                 for (int kb = 0; kb < KB; kb++) s[r][kb] = O::mul(kf[kb], rb[r].ql[ks], s[r][kb]);
         }
     }
+    // The softmax goes ahead of the products of the SIMD's other wave, so that its own products are there sooner to
+    // fill the matrix unit: 2048 tokens behind 6000 253 -> 242 us; with one row block nothing (16.9 and 17.5).
+    if constexpr (RB > 1) __builtin_amdgcn_s_setprio(1);
     // keys key0 + 16 kb + 4 g16 + e of row c16
     constexpr bool low = O::split || LOW;
     V8 ph[RB][KB / 2], pl[low ? RB : 1][KB / 2];
@@ -272,6 +275,7 @@ __device__ __forceinline__ void tile_step(RowBlock<TYPE, HD> (&rb)[RB], const ch
                     pl[r][kb >> 1][4 * (kb & 1) + e] = (typename PagedType<TYPE>::Page)((p - (float)hi) * (O::split ? kLow : 1.0f));
             }
     }
+    if constexpr (RB > 1) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int h = 0; h < KB / 2; h++)
 #pragma unroll
