@@ -440,13 +440,14 @@ int pqa_paged_memory(pqa_paged* p, void** key_pages, void** val_pages, int8_t** 
  * max_pos: pqa_batch_set refuses longer sequences. Synchronous; batches are set again after it.
  * Refused once an append has been captured. */
 int pqa_paged_set_rope(pqa_paged* p, int rope_style, int rot_dim, int max_pos, const float* rope_cos, const float* rope_sin);
-/* QK-RMSNorm weights of one layer, as pqa_set_qk_norm. Synchronous. */
+/* QK-RMSNorm weights of one layer, as pqa_set_qk_norm. Synchronous. A captured append goes on as it was
+ * captured, with or without a norm; new weights reach it. */
 int pqa_paged_set_qk_norm(pqa_paged* p, int layer, const float* q_norm_w, const float* k_norm_w);
 
 /* A batch of at most max_seqs sequences with max_tokens new tokens in all and lengths up to
- * max_len. Holds tables of 4 bytes per page of max_seqs sequences of max_len, and workspaces for
- * cut rows: (2 x 16 x workgroups + up to 2 x 128 x workgroups) rows of head_dim + 2 floats, a
- * workgroup or two per CU (8 + 68 MB at head size 128 on 256 CUs; none of the latter if
+ * max_len (at most 2^30). Holds tables of 4 bytes per page of max_seqs sequences of max_len, and workspaces for
+ * cut rows: (2 x 16 x workgroups + up to 2 x 128 x workgroups) rows of head_dim + 2 floats, one
+ * to three workgroups per CU (2 + 68 MB at head size 128 in 16 bits on 256 CUs; none of the latter if
  * max_tokens query rows of a KV head are 16 or fewer). */
 int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int max_tokens, int max_len);
 /* Waits for the device. */

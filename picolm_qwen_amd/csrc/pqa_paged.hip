@@ -255,6 +255,7 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
         if (!out) return fail(p, PQA_ERR_ARG, name + ": out is NULL");
         *out = nullptr;
         if (max_seqs <= 0 || max_tokens <= 0 || max_len <= 0) return fail(p, PQA_ERR_ARG, name + ": sizes must be positive");
+        if (max_len > (1 << 30)) return fail(p, PQA_ERR_UNSUPPORTED, name + ": max_len above 2^30");  // tiles are counted in 31 bits
         if ((long long)max_tokens * (p->n_heads + 2LL * p->n_kv) * 16 >= (1LL << 31) || max_seqs >= (1 << 24))
             return fail(p, PQA_ERR_UNSUPPORTED, name + ": batch too large");
         pqa_batch* b = new pqa_batch();

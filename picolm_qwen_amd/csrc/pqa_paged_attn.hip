@@ -1072,7 +1072,9 @@ hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q
     const long long grid = captured ? b->shape.narrow_wgs : cols * chosen_parts(a.wgs, (int)cols, select, a.shift);
     // tokens of one sequence share the loads of a choice, and long columns its work: a launch of its own for these
     const bool tokens = captured ? b->shape.max_tokens <= b->shape.max_seqs : ch.single;
-    const bool fused = tokens && ch.parts == 1 && select <= kFusedPages &&
+    // (and where 16 heads are not all: a workgroup of the others may write their rows, which the choice reads,
+    // if out is q)
+    const bool fused = tokens && ch.parts == 1 && p->group <= 16 && select <= kFusedPages &&
                        4 * ch.stride <= narrow_waves(p->head_dim) * 2 * kNarrowKeys * 4 * p->head_dim;
     if (!fused) {
         const hipError_t e = launch_paged_choose(b, ch, captured, s);

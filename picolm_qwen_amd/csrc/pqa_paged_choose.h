@@ -269,7 +269,7 @@ __device__ __forceinline__ void choose_by_block(const Keys& keys, int select, Li
     if (left > 0)
         while (shift > 0) {
             const int width = min(8, shift), next = shift - width;
-            if (tid < 256) s.hist[tid] = 0;
+            for (int i = tid; i < 256; i += threads) s.hist[i] = 0;
             __syncthreads();
             for (int i = p0 + tid; i < p1; i += threads) {
                 const uint32_t k = keys.k[i] - lo;

@@ -54,6 +54,7 @@ class PagedBatch:
     def set(self, n_new, lengths, pages) -> None:
         """n_new[i] new tokens at the end of lengths[i] positions; pages: a list of page lists, or an integer
         array [n_seqs][stride]."""
+        self.att.handle  # a closed cache raises
         n_new, lengths = _int_array(n_new, "n_new"), _int_array(lengths, "lengths")
         if n_new.ndim != 1 or lengths.shape != n_new.shape:
             raise ValueError("n_new and lengths must be lists of one length")
@@ -238,9 +239,10 @@ class PagedAttention:
         self._check(lib().pqa_paged_set_qk_norm(self.handle, layer, *[None if x is None else x.ctypes.data for x in w]))
 
     def batch(self, max_seqs: int, max_tokens: int, max_len=None) -> PagedBatch:
-        """A batch of at most max_seqs sequences and max_tokens new tokens; max_len: the longest sequence (None: the whole pool)."""
+        """A batch of at most max_seqs sequences and max_tokens new tokens; max_len: the longest sequence (None: the whole pool,
+        for which the batch's page table takes 4 * max_seqs * n_pages bytes)."""
         if max_len is None:
-            max_len = min(self.n_pages * self.page_size, 2**31 - 1)
+            max_len = min(self.n_pages * self.page_size, 2**30)
         return PagedBatch(self, max_seqs, max_tokens, max_len)
 
     # -- calls ----------------------------------------------------------------
@@ -274,9 +276,8 @@ class PagedAttention:
         a = self._rows(q, self.q_dim, n, "q")
         if q_out is None:
             q_out = self._out(q, batch)
-        rc = self._calls.pqa_paged_append(self.handle, batch.handle, layer, *a, *self._rows(k, self.kv_dim, n, "k"),
-                                          *self._rows(v, self.kv_dim, n, "v"), *self._rows(q_out, self.q_dim, n, "q_out"),
-                                          self._stream())
+        more = self._rows(k, self.kv_dim, n, "k") + self._rows(v, self.kv_dim, n, "v") + self._rows(q_out, self.q_dim, n, "q_out")
+        rc = self._calls.pqa_paged_append(self.handle, batch.handle, layer, *a, *more, self._stream())
         if rc:
             self._check(rc)
         return q_out
@@ -287,7 +288,8 @@ class PagedAttention:
         a = self._rows(q, self.q_dim, n, "q")
         if out is None:
             out = self._out(q, batch)
-        rc = self._calls.pqa_paged_attend(self.handle, batch.handle, layer, *a, *self._rows(out, self.q_dim, n, "out"), self._stream())
+        o = self._rows(out, self.q_dim, n, "out")
+        rc = self._calls.pqa_paged_attend(self.handle, batch.handle, layer, *a, *o, self._stream())
         if rc:
             self._check(rc)
         return out
@@ -298,8 +300,8 @@ class PagedAttention:
         a = self._rows(q, self.q_dim, n, "q")
         if out is None:
             out = self._out(q, batch)
-        rc = self._calls.pqa_paged_forward(self.handle, batch.handle, layer, *a, *self._rows(k, self.kv_dim, n, "k"),
-                                           *self._rows(v, self.kv_dim, n, "v"), *self._rows(out, self.q_dim, n, "out"), self._stream())
+        more = self._rows(k, self.kv_dim, n, "k") + self._rows(v, self.kv_dim, n, "v") + self._rows(out, self.q_dim, n, "out")
+        rc = self._calls.pqa_paged_forward(self.handle, batch.handle, layer, *a, *more, self._stream())
         if rc:
             self._check(rc)
         return out
@@ -321,8 +323,9 @@ class PagedAttention:
               or tuple(chosen.shape[1:]) != (self.n_kv_heads, select) or not chosen.is_contiguous()
               or chosen.get_device() != self._index):
             raise ValueError(f"chosen must be contiguous int32 [{n}][{self.n_kv_heads}][{select}] on the cache's GPU")
-        rc = self._calls.pqa_paged_attend_sparse(self.handle, batch.handle, layer, *a, select, first, last, chosen.data_ptr(),
-                                                 *self._rows(out, self.q_dim, n, "out"), self._stream())
+        o = self._rows(out, self.q_dim, n, "out")
+        rc = self._calls.pqa_paged_attend_sparse(self.handle, batch.handle, layer, *a, select, first, last, chosen.data_ptr(), *o,
+                                                 self._stream())
         if rc:
             self._check(rc)
         return out, chosen

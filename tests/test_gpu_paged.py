@@ -426,6 +426,40 @@ def test_many_pages_of_one_sequence():
     check_sparse(sparse_case("bf16", (4, 1, 64), 16, [(1, 40000)]), 100, 1, 2)
 
 
+@pytest.mark.parametrize("kind,shape,page,length,select", [
+    ("f16", (2, 1, 256), 16, 20000, 40), ("f32", (4, 2, 192), 16, 17000, 5), ("bf16", (8, 1, 128), 16, 40000, 300)])
+def test_long_lists_of_single_tokens(kind, shape, page, length, select):
+    # more pages than a wave lists, at the head sizes whose workgroups have two waves and four: with a second
+    # sequence, and with so many pages and so few columns that these are shared out
+    check_sparse(sparse_case(kind, shape, page, [(1, length), (1, 700)]), select, 1, 2)
+
+
+@pytest.mark.parametrize("shape", [(34, 2, 64), (34, 1, 128), (8, 2, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("seqs", [[(1, 1500), (1, 900)], [(12, 700), (1, 900)]], ids=["tokens", "chunk"])
+def test_attend_sparse_in_place(shape, seqs):
+    # out is q, also where a KV head's query heads take several workgroups
+    c = sparse_case("f16", shape, 16, seqs)
+    want, chosen = c.att.attend_sparse(0, c.batch, c.q.cuda(), 6, 1, 2)
+    for _ in range(5):
+        q = c.q.cuda()
+        out, again = c.att.attend_sparse(0, c.batch, q, 6, 1, 2, out=q)
+        assert out is q and torch.equal(out, want) and torch.equal(again, chosen)
+
+
+def test_infinities_among_chosen_pages():
+    for kind in ("f32", "bf16"):
+        c = sparse_case(kind, (8, 2, 128), 16, [(1, 900), (5, 700)])
+        for t, at in zip(c.tables, (899, 698)):  # pages that are always chosen: the token's own, and one that three see
+            c.v[0, t[at // 16], 0, at % 16, 7] = float("inf")
+        c.dv.copy_(c.v)
+        got, chosen = c.att.attend_sparse(0, c.batch, c.q.cuda(), 8, 1, 2)
+        got = got.double().cpu().view(c.n, 2, 4, 128)
+        for row in range(c.n):
+            sees = row == 0 or 695 + row - 1 >= 698
+            assert torch.isfinite(got[row, 1]).all()
+            assert bool(torch.isinf(got[row, 0, :, 7]).all()) == sees and torch.isfinite(got[row, 0, :, :7]).all()
+
+
 # ---- a run of them, as a server uses them ----
 
 def test_a_server_step_by_step_against_the_contiguous_cache():
@@ -621,6 +655,36 @@ def test_refusals():
         c.att.append(0, c.batch, q, k, v)
     c.batch.set(c.n_new, c.lengths, c.tables)
     c.att.append(0, c.batch, q, k, v)
+
+
+def test_a_closed_cache_and_its_batches():
+    c = Cache("f16", (4, 2, 64), 16, [(1, 30)], seed=1)
+    c.att.close()
+    for call in (lambda: c.att.attend(0, c.batch, c.q.cuda()), lambda: c.batch.set([1], [30], c.tables)):
+        with pytest.raises(RuntimeError, match="destroyed"):
+            call()
+    c.batch.close()
+    d = Cache("f16", (4, 2, 64), 16, [(1, 30)], seed=1)
+    d.batch.close()
+    with pytest.raises(RuntimeError, match="destroyed"):
+        d.att.attend(0, d.batch, d.q.cuda())
+
+
+def test_calls_run_on_the_current_stream():
+    # behind a long copy on a side stream, which the default stream does not wait for
+    c = Cache("bf16", (8, 2, 128), 16, [(1, 500), (30, 90)], seed=3)
+    want, bound = c.want()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    big = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(s):
+        for _ in range(4):
+            big.add_(1)
+        q = torch.empty_like(c.q, device="cuda")
+        q.copy_(c.q)
+        out = c.att.attend(0, c.batch, q)
+        got = out.cpu()
+    near(got, want, bound)
 
 
 def test_an_empty_batch_launches_nothing():
