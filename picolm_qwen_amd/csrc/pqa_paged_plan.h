@@ -167,14 +167,14 @@ inline PagedFault paged_check(const PagedShape& s, int n_seqs, const int* n_new,
 
 // Which kernel takes a sequence of few rows. Beside chunks the wide one does, as long as its keys are
 // few: one launch, and the chunks' workgroups fill the gaps (3 chunks of 150 to 500 tokens beside 9
-// single ones behind 10 to 4000, 32 / 4 heads of 64: 34.4 us in two launches, 21.2 in one). From
-// kWideBytes on the narrow one's rate is worth its launch (48 tokens behind 345k positions of 32 / 8 heads
-// of 128: 314 us wide, 204 narrow, a difference of 1 us per 13 MB).
+// single ones behind 10 to 4000, fp32, 32 / 4 heads of 64: 30.0 us in two launches, 16.9 in one). From
+// kWideBytes on the narrow one's rate is worth its launch (a chunk of 100 beside 32 tokens behind 3000,
+// bf16, 32 / 8 heads of 128, 393 MB: 83 us in one, 76 in two; behind 8000 188 and 170).
 constexpr long long kWideBytes = 96LL << 20;
-// Without chunks, K and V of this many bytes go past the L2s (32 MB in all), which then keep what the
-// call reads again: 131072 keys of 8 heads of 128 (537 MB) 100 -> 89 us, the 48 tokens above 204 -> 182. Below, a
-// caller that comes back to the same layer soon finds them there: 700 keys of 2 heads of 64 8.4
-// us, past the caches 9.3.
+// K and V of this many bytes and more go past the L2s (32 MB in all), which then keep what the call
+// reads again: 131072 keys of 8 heads of 128 (537 MB) 101 -> 90 us, 48 tokens behind 345k positions 205 ->
+// 183. Below, a caller that comes back to the same layer soon finds them there: 700 keys of 2 heads of
+// 64 8.4 us, past the caches 9.3.
 constexpr long long kStreamBytes = 48LL << 20;
 
 // The narrow items: the key tiles of all (sequence, KV head) columns laid end to end and cut
