@@ -249,11 +249,11 @@ class PagedAttention:
     def _rows(self, t, dim: int, n: int, what: str):
         """(address, row distance) of token rows the library reads or writes n of; anything that would make a kernel leave the
         tensor raises."""
-        shape, stride = t.shape, t.stride()
-        if (len(shape) != 2 or shape[1] != dim or shape[0] < n or stride[1] != 1 or stride[0] < dim
-                or t.dtype is not self.io_type or t.get_device() != self._index):
-            return self._unusual_rows(t, dim, n, what)
-        return t.data_ptr(), stride[0]
+        stride = t.stride()
+        if (len(stride) == 2 and stride[1] == 1 and stride[0] >= dim and t.size(1) == dim and t.size(0) >= n
+                and t.dtype is self.io_type and t.get_device() == self._index):
+            return t.data_ptr(), stride[0]
+        return self._unusual_rows(t, dim, n, what)
 
     def _unusual_rows(self, t, dim: int, n: int, what: str):
         if t.dim() != 2 or t.shape[1] != dim or t.shape[0] < n:
@@ -268,7 +268,11 @@ class PagedAttention:
 
     def _out(self, q, batch):
         # rows behind the batch's last token are not written
-        return self._empty_like(q) if q.shape[0] == batch.n_tokens else self._zeros_like(q)
+        return self._empty_like(q) if q.size(0) == batch.n_tokens else self._zeros_like(q)
+
+    def _handles(self, batch):
+        h, b = self._h, batch._h
+        return (h, b) if h is not None and b is not None else (self.handle, batch.handle)  # the latter raise
 
     def append(self, layer: int, batch: PagedBatch, q, k, v, q_out=None):
         """K and V of the batch's new tokens into their pages; returns q normed and rotated (q_out may be q)."""
@@ -277,7 +281,7 @@ class PagedAttention:
         if q_out is None:
             q_out = self._out(q, batch)
         more = self._rows(k, self.kv_dim, n, "k") + self._rows(v, self.kv_dim, n, "v") + self._rows(q_out, self.q_dim, n, "q_out")
-        rc = self._calls.pqa_paged_append(self.handle, batch.handle, layer, *a, *more, self._stream())
+        rc = self._calls.pqa_paged_append(*self._handles(batch), layer, *a, *more, self._stream())
         if rc:
             self._check(rc)
         return q_out
@@ -289,7 +293,7 @@ class PagedAttention:
         if out is None:
             out = self._out(q, batch)
         o = self._rows(out, self.q_dim, n, "out")
-        rc = self._calls.pqa_paged_attend(self.handle, batch.handle, layer, *a, *o, self._stream())
+        rc = self._calls.pqa_paged_attend(*self._handles(batch), layer, *a, *o, self._stream())
         if rc:
             self._check(rc)
         return out
@@ -301,7 +305,7 @@ class PagedAttention:
         if out is None:
             out = self._out(q, batch)
         more = self._rows(k, self.kv_dim, n, "k") + self._rows(v, self.kv_dim, n, "v") + self._rows(out, self.q_dim, n, "out")
-        rc = self._calls.pqa_paged_forward(self.handle, batch.handle, layer, *a, *more, self._stream())
+        rc = self._calls.pqa_paged_forward(*self._handles(batch), layer, *a, *more, self._stream())
         if rc:
             self._check(rc)
         return out
@@ -324,7 +328,7 @@ class PagedAttention:
               or chosen.get_device() != self._index):
             raise ValueError(f"chosen must be contiguous int32 [{n}][{self.n_kv_heads}][{select}] on the cache's GPU")
         o = self._rows(out, self.q_dim, n, "out")
-        rc = self._calls.pqa_paged_attend_sparse(self.handle, batch.handle, layer, *a, select, first, last, chosen.data_ptr(), *o,
+        rc = self._calls.pqa_paged_attend_sparse(*self._handles(batch), layer, *a, select, first, last, chosen.data_ptr(), *o,
                                                  self._stream())
         if rc:
             self._check(rc)
