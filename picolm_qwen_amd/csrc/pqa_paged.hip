@@ -330,8 +330,8 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         const std::string name = fn;
         if (!b) return fail(nullptr, PQA_ERR_ARG, name + ": batch is NULL");
         pqa_paged* p = b->p;
-        pqa::PagedShape& s = b->shape;
-        s.max_pos = p->max_pos;
+        pqa::PagedShape s = b->shape;
+        s.max_pos = p->max_pos;  // kept with the plan that was checked against it
         if (stride < 0) return fail(p, PQA_ERR_ARG, name + ": stride is negative");
         // a new plan beside the old one, which stays as it is if anything is wrong
         pqa::PagedPlan plan;
@@ -399,6 +399,7 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         if (e != hipSuccess) return hip_fail(p, e, name);
         b->turn ^= 1;
         b->plan = std::move(plan);
+        b->shape.max_pos = s.max_pos;
         b->set = true;
         return PQA_OK;
     });

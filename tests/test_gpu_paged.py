@@ -515,20 +515,24 @@ def test_a_server_step_by_step_against_the_contiguous_cache():
             assert np.array_equal(got.view(torch.int16).numpy().view(np.uint16), rows)
 
 
-def test_captured_steps_follow_later_sets():
-    # one graph of append, attention and attention with a budget; then other lengths, pages and sequences, chunks too
-    kind, shape, page = "bf16", (8, 2, 128), 16
-    cos, sin = rope_table(1e4, 128, 3000)
-    att = PagedAttention(1, 400, page, *shape, dtype=kind, rope_cos=cos, rope_sin=sin, bounds=True)
+@pytest.mark.parametrize("rows,shape", [(64, (8, 2, 128)), (8, (8, 2, 128)), (8, (4, 1, 128))], ids=["chunks", "tokens", "shared"])
+def test_captured_steps_follow_later_sets(rows, shape):
+    # one graph of append, attention and attention with a budget; then other lengths, pages and sequences, chunks too;
+    # for a batch of single tokens (which choose and attend in one launch), and one of long lists and few columns
+    kind, page = "bf16", 16
+    heads, kv, _ = shape
+    top = 20000 if kv == 1 else 3000
+    n_pages = top // page + 220
+    cos, sin = rope_table(1e4, 128, top)
+    att = PagedAttention(1, n_pages, page, *shape, dtype=kind, rope_cos=cos, rope_sin=sin, bounds=True)
     g = torch.Generator(device="cuda").manual_seed(3)
     for x in (att.key_pages, att.val_pages):
         x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
-    rows = 64
-    batch = att.batch(8, rows, 3000)
-    q, k, v = (torch.zeros(rows, n * 128, dtype=torch.bfloat16, device="cuda") for n in (8, 2, 2))
+    batch = att.batch(8, rows, top)
+    q, k, v = (torch.zeros(rows, n * 128, dtype=torch.bfloat16, device="cuda") for n in (heads, kv, kv))
     out, sparse = torch.zeros_like(q), torch.zeros_like(q)
     turned = torch.zeros_like(q)
-    chosen = torch.zeros((rows, 2, 6), dtype=torch.int32, device="cuda")
+    chosen = torch.zeros((rows, kv, 6), dtype=torch.int32, device="cuda")
 
     def step():
         att.append(0, batch, q, k, v, q_out=turned)
@@ -538,7 +542,7 @@ def test_captured_steps_follow_later_sets():
     rng = np.random.default_rng(1)
 
     def fill(seqs):
-        batch.set([n for n, _ in seqs], [length for _, length in seqs], R.page_lists(rng, [length for _, length in seqs], page, 400))
+        batch.set([n for n, _ in seqs], [length for _, length in seqs], R.page_lists(rng, [length for _, length in seqs], page, n_pages))
         for x in (q, k, v):
             x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
 
@@ -550,7 +554,9 @@ def test_captured_steps_follow_later_sets():
         torch.cuda.synchronize()
         graph = Graph(s.cuda_stream, step)
         for seqs in ([(1, 101), (1, 901)], [(1, 7)], [(1, 2900), (1, 1), (1, 450), (1, 17)], [(40, 300), (1, 1500), (20, 20)], [],
-                     [(0, 50), (3, 2500)], [(1, 100)] * 8):
+                     [(0, 50), (3, 2500)], [(1, 100)] * 8, [(1, top)]):
+            if sum(m for m, _ in seqs) > rows:
+                seqs = [(min(m, 1), length) for m, length in seqs]
             fill(seqs)
             n = sum(m for m, _ in seqs)
             for x in (out, sparse, turned):
@@ -651,10 +657,13 @@ def test_refusals():
     for budget in [(0, 0, 1), (4, -1, 2), (4, 1, 0), (4, 3, 2)]:
         with pytest.raises((PQAError, ValueError)):
             s.att.attend_sparse(0, s.batch, s.q.cuda(), *budget)
-    # a changed rotation is met by a batch that was checked against the old one
+    # a changed rotation is met by a batch that was checked against the old one, also after a refused set
     c.att.set_rope(0, 128, 1e4, 30)
-    with pytest.raises(PQAError, match="set the batch again"):
-        c.att.append(0, c.batch, q, k, v)
+    for _ in range(2):
+        with pytest.raises(PQAError, match="set the batch again"):
+            c.att.append(0, c.batch, q, k, v)
+        with pytest.raises(PQAError, match="rotation"):
+            c.batch.set([1], [31], [[0, 1]])
     c.batch.set(c.n_new, c.lengths, c.tables)
     c.att.append(0, c.batch, q, k, v)
 
