@@ -397,7 +397,7 @@ int pqa_set_prefill_precision(pqa_ctx* ctx, int split_q);
  * Token rows: q [n][n_heads * head_dim], k and v [n][n_kv_heads * head_dim], the batch's new
  * tokens sequence by sequence, with a distance between rows in elements (*_stride: a row of a
  * wider array may hold q, k and v side by side). Any alignment of whole elements is taken; 16-byte
- * rows are faster.
+ * rows are faster. Outputs overlap no input, but for an output that is q itself, row for row.
  *
  * Streams: calls run on the hipStream_t given as `stream` (NULL: the default stream), on the
  * handle's device whatever device is current, and are asynchronous. Everything that uses one
@@ -447,7 +447,7 @@ int pqa_paged_set_qk_norm(pqa_paged* p, int layer, const float* q_norm_w, const 
 /* A batch of at most max_seqs sequences with max_tokens new tokens in all and lengths up to
  * max_len (at most 2^30). Holds tables of 4 bytes per page of max_seqs sequences of max_len, and workspaces for
  * cut rows: (2 x 16 x workgroups + up to 2 x 128 x workgroups) rows of head_dim + 2 floats, one
- * to three workgroups per CU (2 + 68 MB at head size 128 in 16 bits on 256 CUs; none of the latter if
+ * to three workgroups per CU (4 + 68 MB at head size 128 in 16 bits on 256 CUs; none of the latter if
  * max_tokens query rows of a KV head are 16 or fewer). */
 int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int max_tokens, int max_len);
 /* Waits for the device. */

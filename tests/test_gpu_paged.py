@@ -436,6 +436,49 @@ def test_long_lists_of_single_tokens(kind, shape, page, length, select):
     check_sparse(sparse_case(kind, shape, page, [(1, length), (1, 700)]), select, 1, 2)
 
 
+def test_budgets_and_lists_beyond_one_workgroup():
+    # more chosen pages than a fused workgroup holds, and more pages than its tiles leave room for
+    check_sparse(sparse_case("f16", (2, 1, 64), 16, [(1, 16 * 2600 + 3), (1, 90)]), 2100, 1, 2)
+    check_sparse(sparse_case("bf16", (2, 1, 64), 16, [(1, 16 * 16500)]), 20, 1, 2)
+
+
+def test_layers_have_their_own_pages_and_bounds():
+    # the same tokens in layers 0 and 2 of three, other ones in layer 1
+    att = PagedAttention(3, 60, 16, 8, 2, 64, dtype="f16", rope_base=1e4, max_pos=600, bounds=True)
+    batch = att.batch(2, 650, 600)
+    rng = np.random.default_rng(3)
+    tables = R.page_lists(rng, [500, 120], 16, 60)
+    batch.set([500, 120], [500, 120], tables)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = [[torch.randn(620, n * 64, generator=g, device="cuda").half() for n in (8, 2, 2)] for _ in range(2)]
+    att.set_qk_norm(1, np.full(64, 2.0), np.full(64, 0.5))
+    outs = []
+    for layer in (0, 1, 2):
+        q = att.append(layer, batch, *x[layer % 2])
+        outs.append((q, att.attend(layer, batch, q), *att.attend_sparse(layer, batch, q, 5)))
+    for a, b, c in zip(*outs):
+        assert torch.equal(a, c) and not torch.equal(a, b)
+    for t in (att.key_pages, att.val_pages, att.key_bounds, att.key_scales):
+        assert torch.equal(t[0], t[2]) and not torch.equal(t[0], t[1])
+
+
+def test_pages_listed_again_and_again():
+    # a list may name a page that is only read many times: more of them than a choice can be made of
+    c = sparse_case("f16", (2, 1, 64), 16, [(1, 16 * 40 + 1)])
+    table = np.concatenate([np.tile(c.tables[0][:40], 820), c.tables[0][40:41]])
+    n = 16 * 820 * 40 + 1
+    batch = c.att.batch(1, 1, n)
+    batch.set([1], [n], table[None])
+    keys, values = (R.rows_of(x[0], table, 0, n) for x in (c.k, c.v))
+    q = c.q.view(2, 64)
+    near(c.att.attend(0, batch, c.q.cuda()).view(2, 64), *R.attention("f16", q, keys, values, torch.tensor([n - 1, n - 1]), 64))
+    with pytest.raises(PQAError, match="32768"):
+        c.att.attend_sparse(0, batch, c.q.cuda(), 8)
+    batch.set([1], [16 * 32767 + 1], np.concatenate([table[:32767], table[-1:]])[None])
+    out, chosen = c.att.attend_sparse(0, batch, c.q.cuda(), 8)
+    assert torch.isfinite(out).all() and chosen[0, 0, -1] == 32767 and bool((chosen[0, 0, 1:] > chosen[0, 0, :-1]).all())
+
+
 @pytest.mark.parametrize("shape", [(34, 2, 64), (34, 1, 128), (8, 2, 128)], ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("seqs", [[(1, 1500), (1, 900)], [(12, 700), (1, 900)]], ids=["tokens", "chunk"])
 def test_attend_sparse_in_place(shape, seqs):
