@@ -281,7 +281,8 @@ extern "C" int pqa_batch_create(pqa_paged* p, pqa_batch** out, int max_seqs, int
         b->max_wide = ((size_t)max_tokens * p->group / s.wide_rows + max_seqs) * p->n_kv + 4 * s.wide_wgs;
         const size_t entries = (size_t)max_seqs * s.max_seq_pages;
         // no plan of this capacity leaves more partials: a block of rows is cut into at most max_len / kWideLeast + 1 parts
-        const size_t blocks = (size_t)max_tokens * p->group <= pqa::kNarrowRows ? 0 : (size_t)max_tokens * p->group / s.least_rows + std::min(max_seqs, max_tokens);
+        const size_t rows = (size_t)max_tokens * p->group;
+        const size_t blocks = rows <= pqa::kNarrowRows ? 0 : rows / s.least_rows + std::min(max_seqs, max_tokens);
         const size_t wide_parts = std::min<size_t>(pqa::paged_wide_slots(s), blocks * p->n_kv * ((size_t)max_len / pqa::kWideLeast + 1));
         struct {
             void** p;
@@ -339,7 +340,8 @@ extern "C" int pqa_batch_set(pqa_batch* b, int n_seqs, const int* n_new, const i
         const PagedFault f = pqa::paged_check(s, n_seqs, n_new, len, pages, stride, &plan, &why);
         if (f != PagedFault::none) return fail(p, f == PagedFault::range ? PQA_ERR_RANGE : PQA_ERR_ARG, name + ": " + why);
         pqa::paged_items(s, &plan);
-        if (plan.runs.size() > (size_t)s.narrow_wgs || plan.rest.size() > b->max_rest || plan.wide.size() > b->max_wide || plan.touched.size() > b->max_touched)
+        if (plan.runs.size() > (size_t)s.narrow_wgs || plan.rest.size() > b->max_rest || plan.wide.size() > b->max_wide ||
+            plan.touched.size() > b->max_touched)
             return fail(p, PQA_ERR_ARG, name + ": plan exceeds the batch");  // cannot happen: the capacities follow from the checks
         OnDevice on(b->device);
         hipStream_t st = (hipStream_t)stream;

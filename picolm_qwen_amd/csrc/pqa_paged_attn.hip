@@ -787,7 +787,8 @@ __device__ __forceinline__ void narrow_body(const PagedAttn& a, const PagedChoos
         for (int kt = tile0; kt < t1; kt += KW) {
             if (kt + KW < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPW < 63 ? LPW : 63) : "memory");  // the next tile's stay in flight
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            tile_step<TYPE, HD, KEYS, 1, KW == narrow_waves(HD)>(rb, lds[w][buf][0], lds[w][buf][1], kt * KEYS, kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
+            tile_step<TYPE, HD, KEYS, 1, KW == narrow_waves(HD)>(rb, lds[w][buf][0], lds[w][buf][1], kt * KEYS,
+                                                                 kt * KEYS + KEYS - 1 > qmin, koff, voff, g16);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer has been read
             issue(kt + 2 * KW, buf);
             buf ^= 1;
@@ -970,15 +971,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : HD <= 128 ? 2 : 1) void paged_w
     }
 }
 
+// Which kernels a call launches, on how many workgroups (0: not at all).
+struct Launch {
+    int narrow_grid, wide_grid;
+    const PagedChoose* choose;  // the narrow kernel makes the choice of its pages, or null
+    bool stream, small, captured;
+};
+
 template <int TYPE, int HD>
-hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
-    if (narrow_grid) {
+hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const Launch& l, hipStream_t s) {
+    if (l.narrow_grid) {
         constexpr int KW = narrow_waves(HD);
-        const dim3 grid((unsigned)narrow_grid);
-        if (ch) {
-            if (stream) hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a, *ch);
-            else hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a, *ch);
-        } else if (stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a);
+        const dim3 grid((unsigned)l.narrow_grid);
+        if (l.choose) {
+            if (l.stream) hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a, *l.choose);
+            else hipLaunchKernelGGL((paged_sparse_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a, *l.choose);
+        } else if (l.stream) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, true>), grid, dim3(64 * KW), 0, s, a);
         else if (a.crowd) hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, 2, false>), grid, dim3(128), 0, s, a);
         else hipLaunchKernelGGL((paged_narrow_kernel<TYPE, HD, KW, false>), grid, dim3(64 * KW), 0, s, a);
         const hipError_t e = hipGetLastError();
@@ -986,34 +994,34 @@ hipError_t launch_kernels(const PagedAttn& a, const PagedAttn& wide, const Paged
     }
     // a captured call launches both tiles; the one that the batch's items are not made for finds none
     constexpr int RB = wide_blocks(TYPE, HD);
-    if (wide_grid && (captured || !small)) {
-        hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, RB>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
+    if (l.wide_grid && (l.captured || !l.small)) {
+        hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, RB>), dim3((unsigned)l.wide_grid), dim3(256), 0, s, wide);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     if constexpr (RB > 1)
-        if (wide_grid && (captured || small)) {
-            hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, 1>), dim3((unsigned)wide_grid), dim3(256), 0, s, wide);
+        if (l.wide_grid && (l.captured || l.small)) {
+            hipLaunchKernelGGL((paged_wide_kernel<TYPE, HD, 1>), dim3((unsigned)l.wide_grid), dim3(256), 0, s, wide);
             return hipGetLastError();
         }
     return hipSuccess;
 }
 
 template <int TYPE>
-hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_type(int hd, const PagedAttn& a, const PagedAttn& wide, const Launch& l, hipStream_t s) {
     switch (hd) {
-#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
+#define PQA_PG(H) case H: return launch_kernels<TYPE, H>(a, wide, l, s);
         PQA_PG(64) PQA_PG(96) PQA_PG(128) PQA_PG(160) PQA_PG(192) PQA_PG(256)
 #undef PQA_PG
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, const PagedChoose* ch, bool stream, bool small, bool captured, int narrow_grid, int wide_grid, hipStream_t s) {
+hipError_t launch_any(const pqa_batch* b, const PagedAttn& a, const PagedAttn& wide, const Launch& l, hipStream_t s) {
     switch (b->p->type) {
-        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
-        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
-        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, ch, stream, small, captured, narrow_grid, wide_grid, s);
+        case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(b->p->head_dim, a, wide, l, s);
+        case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(b->p->head_dim, a, wide, l, s);
+        default: return launch_type<PQA_PAGED_BF16>(b->p->head_dim, a, wide, l, s);
     }
 }
 
@@ -1063,7 +1071,7 @@ hipError_t launch_paged_attend(const pqa_batch* b, int layer, const PagedRows& q
     // any content fits
     const int n = captured ? b->shape.narrow_wgs : (int)b->plan.runs.size();
     const int w = captured ? b->shape.wide_wgs : (int)b->plan.wide.size();
-    return launch_any(b, a, wide, nullptr, b->plan.stream, b->plan.wide_rows < b->shape.wide_rows, captured, n, w, s);
+    return launch_any(b, a, wide, {n, w, nullptr, b->plan.stream, b->plan.wide_rows < b->shape.wide_rows, captured}, s);
 }
 
 hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q, int select, int first, int last, int* chosen,
@@ -1088,7 +1096,7 @@ hipError_t launch_paged_sparse(const pqa_batch* b, int layer, const PagedRows& q
     a.crowd = !fused && cols >= 2 * a.wgs;
     // chosen pages of single tokens are read once, those of a chunk's tokens by many of them
     const bool stream = ch.single && cols * ((long long)select << a.shift) * 4 * p->head_dim > kStreamBytes;
-    return launch_any(b, a, a, fused ? &ch : nullptr, stream, false, captured, (int)std::min<long long>(grid, 1 << 30), 0, s);
+    return launch_any(b, a, a, {(int)std::min<long long>(grid, 1 << 30), 0, fused ? &ch : nullptr, stream, false, captured}, s);
 }
 
 }  // namespace pqa

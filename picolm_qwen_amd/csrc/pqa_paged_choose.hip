@@ -146,7 +146,8 @@ hipError_t launch_paged_choose(const pqa_batch* b, const PagedChoose& a, bool ca
     const pqa_paged* p = b->p;
     const size_t lds = (size_t)a.group * a.stride * 4;
     const long long most = 16LL * p->cu_count;
-    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(1 << 30, ((long long)b->plan.n_tok + a.group) * p->n_kv * a.parts));
+    const long long units = ((long long)b->plan.n_tok + a.group) * p->n_kv * a.parts;
+    const unsigned grid = (unsigned)(captured ? most : std::min<long long>(1 << 30, units));
     switch (p->type) {
         case PQA_PAGED_F32: return launch_type<PQA_PAGED_F32>(p->head_dim, a, grid, lds, s);
         case PQA_PAGED_F16: return launch_type<PQA_PAGED_F16>(p->head_dim, a, grid, lds, s);

@@ -115,7 +115,11 @@ class PagedAttention:
         given = [x is not None for x in (key_pages, val_pages)]
         if any(given) != all(given) or (key_bounds is None) != (key_scales is None) or (key_bounds is not None and not all(given)):
             raise ValueError("give key_pages and val_pages together, and key_bounds and key_scales with them")
-        device = key_pages.device if all(given) else torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else None
+        device = None
+        if all(given):
+            device = key_pages.device
+        elif torch.cuda.is_available():
+            device = torch.device("cuda", torch.cuda.current_device())
         shape = (n_layers, n_pages, n_kv_heads)
         if all(given):
             for t, tail, kind, what in ((key_pages, (page_size, head_dim), self.page_type, "key_pages"),
